@@ -68,6 +68,18 @@ void mem_grid(const Variant &v, const dnxcu_dispatch &d, uint32_t g[3]);
 // Limit of every bounded device-side wait in clock64 ticks (dnxcu_set_wait_limit_us).
 unsigned long long wait_limit_cycles();
 
+// ---- token and pixel operators ---------------------------------------------
+// A matrix of `rows` rows of `len` elements of `es` bytes, `stride` elements apart, for the argument checks.
+struct RowSpan {
+  const void *p;
+  long long rows, len, stride;
+  int es;
+};
+// Whether two row spans share a byte (exactly equal spans do; windows side by side in the same wider rows do not).
+bool rows_overlap(const RowSpan &a, const RowSpan &b);
+// Whether kernels on the current device may use the pointer: memory of this device, managed or registered host memory.
+bool on_current_device(const void *p);
+
 // SHA-256 (hex) of a byte string; used for variant identities and database keys.
 void sha256_hex(const void *data, size_t n, char out_hex[65]);
 

@@ -1,0 +1,429 @@
+// Root-mean-square norm over the channels of each row, with the residual's addition in front and, on request, an
+// 8 bit output with one scale per row.
+//
+//   h = x + residual,  y = weight * h / sqrt(mean(h^2) + eps)
+//   8 bits:  scale = max|y| / 448,  q = y / scale
+//
+// One pass over the data: a row's elements stay in registers between the statistics and the output.  The row's
+// largest |y| needs no second reduction: 1 / rms is a positive constant of the row, so max|y| = max|weight * h| / rms
+// is taken beside the sum of squares, and q = (weight * h) * (448 / max|weight * h|) does not need rms at all.
+// The maximum is taken on the absolute values' bit patterns, whose unsigned order is the values' order with NaN
+// above infinity: a row that is not finite shows in it, and one integer `redux` does a warp's.
+//
+// Bound by bytes.  Four forms, by the row's length and by what the alignment allows (V elements per access, 16 bytes
+// where every pointer and stride is a multiple of that):
+//   warp form  rows of at most 1024 channels: a power of two of lanes per row, several rows per warp; every thread
+//              has 32 elements in flight whatever the row's length (U rows of E elements, U * E = 32);
+//   block form rows up to 32 elements x 1024 threads: a block per row;
+//   loop form  anything longer (or long and unaligned): a block per row that reads it twice, the second time from L2.
+#include "internal.h"
+#include <cuda_fp8.h>
+#include <math.h>
+
+namespace dnxcu {
+namespace {
+
+struct NormArgs {
+  const __half *x, *residual, *weight;
+  __half *sum;
+  void *out;
+  float *scale;
+  long long rows, xs, rs, ss, os;  // strides in elements
+  int C;
+  float eps, inv_c;
+};
+
+template <int V> struct Vec;
+template <> struct Vec<8> { typedef uint4 H; typedef uint2 Q; };
+template <> struct Vec<4> { typedef uint2 H; typedef uint32_t Q; };
+template <> struct Vec<2> { typedef uint32_t H; typedef uint16_t Q; };
+template <> struct Vec<1> { typedef uint16_t H; typedef uint8_t Q; };
+
+template <int V>
+union Halves {
+  typename Vec<V>::H v;
+  __half h[V];
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Loads of data that an output of the same call may alias are plain loads (never the read-only path); every thread
+// reads an element before it writes it, and no thread reads another's.
+template <int V>
+__device__ __forceinline__ void load_sum(const NormArgs &g, long long row, int c, float (&h)[V]) {
+  Halves<V> a;
+  a.v = *reinterpret_cast<const typename Vec<V>::H *>(g.x + row * g.xs + c);
+#pragma unroll
+  for (int e = 0; e < V; ++e) h[e] = __half2float(a.h[e]);
+  if (g.residual) {
+    a.v = *reinterpret_cast<const typename Vec<V>::H *>(g.residual + row * g.rs + c);
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[e] += __half2float(a.h[e]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void load_weight(const NormArgs &g, int c, float (&w)[V]) {
+  if (g.weight) {
+    Halves<V> a;
+    a.v = __ldg(reinterpret_cast<const typename Vec<V>::H *>(g.weight + c));
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = __half2float(a.h[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = 1.0f;
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_sum(const NormArgs &g, long long row, int c, const float (&h)[V]) {
+  Halves<V> a;
+#pragma unroll
+  for (int e = 0; e < V; ++e) a.h[e] = __float2half_rn(h[e]);
+  *reinterpret_cast<typename Vec<V>::H *>(g.sum + row * g.ss + c) = a.v;
+}
+// y = weight * h * f, rounded once to the output type.  8 bits: f = 448 / max|weight * h|; a product that the last
+// bit of f puts above 448 saturates to it.
+template <int V, bool Q>
+__device__ __forceinline__ void store_out(const NormArgs &g, long long row, int c, const float (&h)[V], const float (&w)[V],
+                                          float f) {
+  if (Q) {
+    union {
+      typename Vec<V>::Q v;
+      uint8_t b[V];
+    } q;
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.b[e] = __nv_cvt_float_to_fp8(h[e] * w[e] * f, __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<typename Vec<V>::Q *>((uint8_t *)g.out + row * g.os + c) = q.v;
+  } else {
+    Halves<V> a;
+#pragma unroll
+    for (int e = 0; e < V; ++e) a.h[e] = __float2half_rn(h[e] * f * w[e]);
+    *reinterpret_cast<typename Vec<V>::H *>((__half *)g.out + row * g.os + c) = a.v;
+  }
+}
+// The row's factor from its statistics; `top` = bits of max|weight * h|.
+template <bool Q>
+__device__ __forceinline__ float row_factor(const NormArgs &g, float ss, uint32_t top, float *scale) {
+  const float rstd = 1.0f / sqrtf(ss * g.inv_c + g.eps);
+  if (!Q) return rstd;
+  if (top >= 0x7f800000u) {  // a value that is not finite: the whole row is NaN
+    *scale = __uint_as_float(0x7fffffffu);
+    return *scale;
+  }
+  if (top == 0) {
+    *scale = 1.0f;
+    return 0.0f;
+  }
+  *scale = __uint_as_float(top) * rstd * (1.0f / 448.0f);
+  return 448.0f / __uint_as_float(top);
+}
+
+// ---- warp form --------------------------------------------------------------
+// 2^LT lanes per row; a thread holds vectors t, t + 2^LT, ... of U rows.
+template <int V, int E, bool Q>
+__global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
+  constexpr int N = E / V, U = 32 / E;
+  const int tpr = 1 << lt, t = threadIdx.x & (tpr - 1);
+  const int per_block = (int)blockDim.x >> lt;
+  const long long rows_per_block = (long long)per_block * U;
+  const int nv = g.C / V;
+  for (long long r0 = (long long)blockIdx.x * rows_per_block; r0 < g.rows; r0 += (long long)gridDim.x * rows_per_block) {
+    float h[U][N][V];
+    long long row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      row[u] = r0 + (long long)u * per_block + (threadIdx.x >> lt);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int vi = t + (i << lt);
+        if (row[u] < g.rows && vi < nv) {
+          load_sum<V>(g, row[u], vi * V, h[u][i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) h[u][i][e] = 0.0f;
+        }
+      }
+    }
+    float w[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int vi = t + (i << lt);
+      if (vi < nv) load_weight<V>(g, vi * V, w[i]);
+      else
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[i][e] = 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float ss = 0.0f;
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          ss = fmaf(h[u][i][e], h[u][i][e], ss);
+          if (Q) top = max(top, abs_bits(h[u][i][e] * w[i][e]));
+        }
+      for (int o = tpr >> 1; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (Q) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
+      if (row[u] >= g.rows) continue;  // (no shuffle follows for this row)
+      float scale = 0.0f;
+      const float f = row_factor<Q>(g, ss, top, &scale);
+      if (Q && t == 0) g.scale[row[u]] = scale;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int vi = t + (i << lt);
+        if (vi < nv) {
+          if (g.sum) store_sum<V>(g, row[u], vi * V, h[u][i]);
+          store_out<V, Q>(g, row[u], vi * V, h[u][i], w[i], f);
+        }
+      }
+    }
+  }
+}
+
+// Sum and maximum over the block; every thread gets both.  `turn` alternates between two halves of the buffer so that
+// one barrier per row is enough.
+__device__ __forceinline__ void block_reduce(float &ss, uint32_t &top, int turn) {
+  __shared__ float s_sum[2][32];
+  __shared__ uint32_t s_top[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (int)blockDim.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) {
+    s_sum[turn][warp] = ss;
+    s_top[turn][warp] = top;
+  }
+  __syncthreads();
+  ss = lane < nw ? s_sum[turn][lane] : 0.0f;
+  top = lane < nw ? s_top[turn][lane] : 0u;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  top = __reduce_max_sync(0xffffffffu, top);
+}
+
+// ---- block form -------------------------------------------------------------
+template <int V, int E, bool Q>
+__global__ void __launch_bounds__(1024) rmsnorm_block(NormArgs g) {
+  constexpr int N = E / V;
+  const int nv = g.C / V, t = threadIdx.x, nt = blockDim.x;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < g.rows; row += gridDim.x, turn ^= 1) {
+    float h[N][V];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int vi = t + i * nt;
+      if (vi < nv) {
+        load_sum<V>(g, row, vi * V, h[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[i][e] = 0.0f;
+      }
+    }
+    float ss = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float w[V];
+      const int vi = t + i * nt;
+      if (Q && vi < nv) load_weight<V>(g, vi * V, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        ss = fmaf(h[i][e], h[i][e], ss);
+        if (Q && vi < nv) top = max(top, abs_bits(h[i][e] * w[e]));
+      }
+    }
+    block_reduce(ss, top, turn);
+    float scale = 0.0f;
+    const float f = row_factor<Q>(g, ss, top, &scale);
+    if (Q && t == 0) g.scale[row] = scale;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int vi = t + i * nt;
+      if (vi < nv) {
+        float w[V];
+        load_weight<V>(g, vi * V, w);  // (from L1: every row uses the same ones)
+        if (g.sum) store_sum<V>(g, row, vi * V, h[i]);
+        store_out<V, Q>(g, row, vi * V, h[i], w, f);
+      }
+    }
+  }
+}
+
+// ---- loop form --------------------------------------------------------------
+template <int V, bool Q>
+__global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
+  const int nv = g.C / V, t = threadIdx.x, nt = blockDim.x;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < g.rows; row += gridDim.x, turn ^= 1) {
+    float ss = 0.0f;
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int vi = t; vi < nv; vi += nt) {
+      float h[V], w[V];
+      load_sum<V>(g, row, vi * V, h);
+      if (Q) load_weight<V>(g, vi * V, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        ss = fmaf(h[e], h[e], ss);
+        if (Q) top = max(top, abs_bits(h[e] * w[e]));
+      }
+    }
+    block_reduce(ss, top, turn);
+    float scale = 0.0f;
+    const float f = row_factor<Q>(g, ss, top, &scale);
+    if (Q && t == 0) g.scale[row] = scale;
+#pragma unroll 4
+    for (int vi = t; vi < nv; vi += nt) {
+      float h[V], w[V];
+      load_sum<V>(g, row, vi * V, h);
+      load_weight<V>(g, vi * V, w);
+      if (g.sum) store_sum<V>(g, row, vi * V, h);
+      store_out<V, Q>(g, row, vi * V, h, w, f);
+    }
+  }
+}
+
+constexpr unsigned kMaxGrid = 0x7fffffffu;
+
+template <int V, bool Q>
+void launch_v(const NormArgs &g, cudaStream_t s) {
+  const int nv = g.C / V;
+  if (g.C <= 1024) {
+    // the fewest lanes (a power of two) that hold the row in 8, 16 or 32 elements per thread, most rows per warp first
+    const int e = g.C <= 256 ? 8 : g.C <= 512 ? 16 : 32;
+    int lt = 0;
+    while ((e / V) << lt < nv) ++lt;
+    const long long per_block = (256 >> lt) * (32 / e);
+    const long long blocks = (g.rows + per_block - 1) / per_block;
+    const unsigned grid = (unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid);
+    if (e == 8) rmsnorm_warp<V, 8, Q><<<grid, 256, 0, s>>>(g, lt);
+    else if (e == 16) rmsnorm_warp<V, 16, Q><<<grid, 256, 0, s>>>(g, lt);
+    else rmsnorm_warp<V, 32, Q><<<grid, 256, 0, s>>>(g, lt);
+    return;
+  }
+  const unsigned grid = (unsigned)(g.rows < kMaxGrid ? g.rows : kMaxGrid);
+  const auto threads = [&](int e) {
+    const int n = e / V, t = (nv + n - 1) / n;
+    return (t + 31) / 32 * 32;
+  };
+  // few rows: as many threads per row as there are, for latency; many rows: 32 elements in flight per thread
+  if (g.rows <= 148 && threads(8) <= 1024) rmsnorm_block<V, 8, Q><<<grid, threads(8), 0, s>>>(g);
+  else if (g.rows <= 148 && threads(16) <= 1024) rmsnorm_block<V, 16, Q><<<grid, threads(16), 0, s>>>(g);
+  else if (threads(32) <= 1024) rmsnorm_block<V, 32, Q><<<grid, threads(32), 0, s>>>(g);
+  else rmsnorm_loop<V, Q><<<grid, 1024, 0, s>>>(g);
+}
+
+template <int V>
+void launch_q(const NormArgs &g, bool q, cudaStream_t s) {
+  if (q) launch_v<V, true>(g, s);
+  else launch_v<V, false>(g, s);
+}
+
+// The record with packed strides filled in, or why it cannot run.
+int check(const dnxcu_rmsnorm *d, NormArgs *g) {
+  if (!d || !d->x || !d->out || d->rows <= 0 || d->channels <= 0 || d->reserved) return DNXCU_E_BAD_ARG;
+  if (d->out_dtype != DNXCU_DT_F16 && d->out_dtype != DNXCU_DT_E4M3) return DNXCU_E_BAD_ARG;
+  const bool q = d->out_dtype == DNXCU_DT_E4M3;
+  if (q != (d->out_scale != nullptr)) return DNXCU_E_BAD_ARG;
+  if (!(d->eps > 0.0f) || !isfinite(d->eps)) return DNXCU_E_BAD_ARG;
+  const long long C = d->channels, kStride = 1ll << 35;
+  if (d->rows > 0x7fffffffll || C > (1 << 24)) return DNXCU_E_LIMIT;
+  const long long xs = d->x_stride ? d->x_stride : C, rs = d->residual_stride ? d->residual_stride : C;
+  const long long ss = d->sum_stride ? d->sum_stride : C, os = d->out_stride ? d->out_stride : C;
+  if (xs < C || rs < C || ss < C || os < C) return DNXCU_E_BAD_ARG;
+  if (xs >= kStride || rs >= kStride || ss >= kStride || os >= kStride) return DNXCU_E_LIMIT;
+  const uintptr_t halves = (uintptr_t)d->x | (uintptr_t)d->residual | (uintptr_t)d->weight | (uintptr_t)d->sum_out |
+                           (q ? 0 : (uintptr_t)d->out);
+  if ((halves & 1) || ((uintptr_t)d->out_scale & 3)) return DNXCU_E_MISALIGNED;
+  const RowSpan x{d->x, d->rows, C, xs, 2}, res{d->residual, d->rows, C, rs, 2}, w{d->weight, 1, C, C, 2};
+  const RowSpan sum{d->sum_out, d->rows, C, ss, 2}, out{d->out, d->rows, C, os, q ? 1 : 2};
+  const RowSpan sc{d->out_scale, 1, d->rows, d->rows, 4};
+  const auto same = [](const RowSpan &a, const RowSpan &b) { return a.p == b.p && a.stride == b.stride && a.es == b.es; };
+  const auto clash = [&](const RowSpan &o, const RowSpan &in) { return !same(o, in) && rows_overlap(o, in); };
+  if (clash(sum, x) || clash(sum, res) || clash(out, x) || clash(out, res)) return DNXCU_E_BAD_ARG;
+  if (rows_overlap(sum, w) || rows_overlap(out, w) || rows_overlap(sum, out)) return DNXCU_E_BAD_ARG;
+  if (rows_overlap(sc, x) || rows_overlap(sc, res) || rows_overlap(sc, w) || rows_overlap(sc, sum) || rows_overlap(sc, out))
+    return DNXCU_E_BAD_ARG;
+  g->x = (const __half *)d->x;
+  g->residual = (const __half *)d->residual;
+  g->weight = (const __half *)d->weight;
+  g->sum = (__half *)d->sum_out;
+  g->out = d->out;
+  g->scale = d->out_scale;
+  g->rows = d->rows;
+  g->C = d->channels;
+  g->xs = xs;
+  g->rs = rs;
+  g->ss = ss;
+  g->os = os;
+  g->eps = d->eps;
+  g->inv_c = (float)(1.0 / (double)C);
+  return DNXCU_OK;
+}
+
+}  // namespace
+
+bool rows_overlap(const RowSpan &a, const RowSpan &b) {
+  if (!a.p || !b.p) return false;
+  const long long sa = a.stride * a.es, sb = b.stride * b.es, la = a.len * a.es, lb = b.len * b.es;
+  const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
+  const uintptr_t a1 = a0 + (uintptr_t)((a.rows - 1) * sa + la), b1 = b0 + (uintptr_t)((b.rows - 1) * sb + lb);
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (sa != sb || a.rows < 2 || b.rows < 2) return true;  // (two interleaved spans of different pitch: taken as overlapping)
+  // same pitch: windows of the same wider rows; b's start within a's row, wrapped into one pitch
+  const long long d = b0 >= a0 ? (long long)((b0 - a0) % (uintptr_t)sa) : (sa - (long long)((a0 - b0) % (uintptr_t)sa)) % sa;
+  return d < la || d + lb > sa;
+}
+
+bool on_current_device(const void *p) {
+  if (!p) return true;
+  cudaPointerAttributes at;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (at.type == cudaMemoryTypeDevice) return at.device == dev;
+  return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeHost && at.devicePointer == p);
+}
+
+}  // namespace dnxcu
+
+using namespace dnxcu;
+
+extern "C" {
+
+int dnxcu_rmsnorm_validate(const dnxcu_rmsnorm *d) {
+  NormArgs g;
+  return check(d, &g);
+}
+
+int dnxcu_rmsnorm_launch(const dnxcu_rmsnorm *d, void *stream) {
+  NormArgs g;
+  const int st = check(d, &g);
+  if (st) return st;
+  if (!on_current_device(g.x) || !on_current_device(g.residual) || !on_current_device(g.weight) ||
+      !on_current_device(g.sum) || !on_current_device(g.out) || !on_current_device(g.scale))
+    return DNXCU_E_BAD_ARG;
+  const bool q = d->out_dtype == DNXCU_DT_E4M3;
+  // elements per access: what every pointer, stride and the row length are multiples of
+  const auto fits = [&](int v) {
+    const uintptr_t hb = (uintptr_t)v * 2 - 1, ob = (uintptr_t)v * (q ? 1 : 2) - 1;
+    if (g.C % v || ((uintptr_t)g.x & hb) || g.xs % v || ((uintptr_t)g.weight & hb)) return false;
+    if (g.residual && (((uintptr_t)g.residual & hb) || g.rs % v)) return false;
+    if (g.sum && (((uintptr_t)g.sum & hb) || g.ss % v)) return false;
+    return !((uintptr_t)g.out & ob) && g.os % v == 0;
+  };
+  cudaStream_t s = (cudaStream_t)stream;
+  if (fits(8)) launch_q<8>(g, q, s);
+  else if (fits(4)) launch_q<4>(g, q, s);
+  else if (fits(2)) launch_q<2>(g, q, s);
+  else launch_q<1>(g, q, s);
+  DNXCU_CUDA(cudaGetLastError());
+  return DNXCU_OK;
+}
+
+}  // extern "C"

@@ -27,6 +27,8 @@ OP_CONV3X3, OP_MAXPOOL2X2, OP_UPSAMPLE2X, OP_CONCAT, OP_RELU, OP_PAD_CHANNELS, O
 F_RELU, F_BIAS, F_UP2X_A, F_POOL_OUT, F_NO_FULL_OUT, F_LEAKY = 0x01, 0x02, 0x04, 0x08, 0x10, 0x20
 OPT_NO_FUSE_ACTIVATION, OPT_NO_FUSE_POOL, OPT_NO_FUSE_UPSAMPLE, OPT_NO_FUSE_CONCAT, OPT_NO_TCGEN05 = 1, 2, 4, 8, 16
 OPT_NO_PAD_INPUT = 32
+DT_F16, DT_E4M3 = 0, 1
+ACT_NONE, ACT_RELU, ACT_LEAKY, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(6)
 OPT_SELECT_BY_COST_ONLY = 64
 
 
@@ -100,6 +102,13 @@ class HaloPoint(C.Structure):
                 ("row_bytes", C.c_uint64)]
 
 
+class RmsNorm(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("channels", C.c_int32), ("out_dtype", C.c_int32), ("eps", C.c_float),
+                ("reserved", C.c_uint32), ("x", C.c_void_p), ("x_stride", C.c_int64), ("residual", C.c_void_p),
+                ("residual_stride", C.c_int64), ("weight", C.c_void_p), ("sum_out", C.c_void_p),
+                ("sum_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64), ("out_scale", C.c_void_p)]
+
+
 # every symbol include/dnxcu.h declares, with its C signature
 SIGNATURES = {
     "dnxcu_status_string": (C.c_char_p, [C.c_int]),
@@ -122,6 +131,8 @@ SIGNATURES = {
                                         C.POINTER(C.c_size_t)]),
     "dnxcu_conv3x3_pool_static": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                             C.c_uint32, C.c_void_p, C.c_void_p]),
+    "dnxcu_rmsnorm_validate": (C.c_int, [C.POINTER(RmsNorm)]),
+    "dnxcu_rmsnorm_launch": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p]),
     "dnxcu_f16_from_float": (C.c_uint16, [C.c_float]),
     "dnxcu_f16_to_float": (C.c_float, [C.c_uint16]),
     "dnxcu_model_create": (C.c_int, [C.POINTER(ModelDesc), C.c_void_p, C.c_int, C.POINTER(C.c_void_p)]),
@@ -257,6 +268,18 @@ def _model_desc(net, options=0):
     desc = ModelDesc(len(net.nodes), net.n_tensors, arr, net.input_tensor, net.in_channels, net.output_tensor,
                      options)
     return desc, keep
+
+
+def rmsnorm_desc(rows, channels, x, out, out_dtype=DT_F16, eps=1e-5, residual=None, weight=None, sum_out=None,
+                 out_scale=None, x_stride=0, residual_stride=0, sum_stride=0, out_stride=0) -> RmsNorm:
+    """Record of a root-mean-square norm (device pointers as integers; strides in elements, 0 = packed rows)."""
+    return RmsNorm(rows, channels, out_dtype, eps, 0, x, x_stride, residual, residual_stride, weight, sum_out, sum_stride,
+                   out, out_stride, out_scale)
+
+
+def rmsnorm(desc: RmsNorm, stream: int = 0):
+    """Enqueues the norm on `stream`."""
+    check(L.dnxcu_rmsnorm_launch(desc, stream), "dnxcu_rmsnorm_launch")
 
 
 class Db:

@@ -245,6 +245,73 @@ DNXCU_API int dnxcu_prepare_weights(int variant, const void *kcrs_f16, int c_out
 DNXCU_API int dnxcu_conv3x3_pool_static(const void *in, int height, int width, int c_in, const void *weights,
                                         const void *bias, int c_out, uint32_t flags, void *out_pool, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Token and pixel operators: the linear layer and the root-mean-square norm.
+ * No counterpart in the reference, whose layers are 3x3 convolutions; these
+ * are what a U-Net with pointwise (1x1) convolutions or with token layers at
+ * its bottleneck needs next to them.  A row is a token, or a pixel of an HWC
+ * tensor (rows = H * W); the row's elements are its channels.
+ *
+ *  - strides are elements from one row to the next; 0 means packed (the row's
+ *    own length).  Rows may be windows of wider rows (stride > length);
+ *  - the entry points check the record before anything is enqueued:
+ *    DNXCU_E_BAD_ARG (null pointer, non-positive size, unknown enum, stride
+ *    below the row length, operands that overlap where they may not, a buffer
+ *    that the current device does not hold), DNXCU_E_MISALIGNED (a pointer
+ *    that is not a multiple of its element), DNXCU_E_LIMIT (a size above the
+ *    limits below), DNXCU_E_UNSUPPORTED (a forced variant that cannot run it);
+ *  - launches are stream ordered, never synchronise, allocate nothing, keep
+ *    nothing between calls and may be captured into a graph; the stream
+ *    belongs to the current device, which also holds every buffer;
+ *  - results do not depend on timing: the same call gives the same bits.
+ * Limits: rows <= 2^31 - 1, channels <= 2^24, row strides < 2^35 elements.
+ * ---------------------------------------------------------------------- */
+typedef enum dnxcu_dtype {
+  DNXCU_DT_F16 = 0,  /* binary16 */
+  DNXCU_DT_E4M3 = 1  /* 8 bit float, 4 exponent and 3 mantissa bits, largest value 448, no infinity */
+} dnxcu_dtype;
+
+typedef enum dnxcu_activation {
+  DNXCU_ACT_NONE = 0,
+  DNXCU_ACT_RELU = 1,      /* max(v, 0) */
+  DNXCU_ACT_LEAKY = 2,     /* v > 0 ? v : leaky_alpha * v */
+  DNXCU_ACT_GELU = 3,      /* v / 2 * (1 + erf(v / sqrt(2))) */
+  DNXCU_ACT_GELU_TANH = 4, /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
+  DNXCU_ACT_SILU = 5       /* v / (1 + exp(-v)) */
+} dnxcu_activation;
+
+/* Root-mean-square norm over the channels of each row, after the residual's addition:
+ *   h   = x + residual                              (h = x without a residual)
+ *   y   = weight * h / sqrt(mean(h^2) + eps)        (weight = 1 without one)
+ *   sum_out = h rounded to binary16                 (when sum_out is given)
+ *   out = y rounded to binary16, or, with out_dtype DNXCU_DT_E4M3,
+ *   out_scale[row] = max|y| / 448 (1 for a row of zeros), out = y / out_scale[row] rounded to e4m3.
+ * Sums, statistics and y are held in 32 bits; y comes from the sum before it is rounded.  A row that holds a NaN
+ * or an infinity has, with an 8 bit output, NaN in all of out and in out_scale; with a binary16 output what the
+ * formula gives (other rows are untouched by it).
+ * sum_out may be x or residual itself, and a binary16 out may be x or residual itself (same pointer and stride);
+ * no other output may overlap an input or another output. */
+typedef struct dnxcu_rmsnorm {
+  int64_t rows;
+  int32_t channels;
+  int32_t out_dtype; /* dnxcu_dtype */
+  float eps;         /* > 0 */
+  uint32_t reserved; /* 0 */
+  const void *x;     /* binary16 */
+  int64_t x_stride;
+  const void *residual; /* binary16, or NULL */
+  int64_t residual_stride;
+  const void *weight; /* binary16 [channels], or NULL */
+  void *sum_out;      /* binary16, or NULL */
+  int64_t sum_stride;
+  void *out; /* out_dtype */
+  int64_t out_stride;
+  float *out_scale; /* [rows] with DNXCU_DT_E4M3, else NULL */
+} dnxcu_rmsnorm;
+
+DNXCU_API int dnxcu_rmsnorm_validate(const dnxcu_rmsnorm *d);
+DNXCU_API int dnxcu_rmsnorm_launch(const dnxcu_rmsnorm *d, void *stream);
+
 /* float -> binary16 exactly as the reference converts fp32 model weights:
  * mantissa truncated, sub-normal results flushed to zero
  * (common/src/denox/memory/dtype/f16.cpp:6-20). */
