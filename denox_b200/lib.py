@@ -29,6 +29,7 @@ OPT_NO_FUSE_ACTIVATION, OPT_NO_FUSE_POOL, OPT_NO_FUSE_UPSAMPLE, OPT_NO_FUSE_CONC
 OPT_NO_PAD_INPUT = 32
 DT_F16, DT_E4M3 = 0, 1
 ACT_NONE, ACT_RELU, ACT_LEAKY, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(6)
+LINEAR_AUTO, LINEAR_ROWS, LINEAR_SPLIT, LINEAR_TILE, LINEAR_ANY = range(5)
 OPT_SELECT_BY_COST_ONLY = 64
 
 
@@ -109,6 +110,15 @@ class RmsNorm(C.Structure):
                 ("sum_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64), ("out_scale", C.c_void_p)]
 
 
+class Linear(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("c_in", C.c_int32), ("c_out", C.c_int32), ("dtype", C.c_int32),
+                ("activation", C.c_int32), ("leaky_alpha", C.c_float), ("variant", C.c_int32), ("x", C.c_void_p),
+                ("x_stride", C.c_int64), ("weights", C.c_void_p), ("w_stride", C.c_int64), ("x_scale", C.c_void_p),
+                ("w_scale", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p),
+                ("residual_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("device_status", C.c_void_p)]
+
+
 # every symbol include/dnxcu.h declares, with its C signature
 SIGNATURES = {
     "dnxcu_status_string": (C.c_char_p, [C.c_int]),
@@ -133,6 +143,12 @@ SIGNATURES = {
                                             C.c_uint32, C.c_void_p, C.c_void_p]),
     "dnxcu_rmsnorm_validate": (C.c_int, [C.POINTER(RmsNorm)]),
     "dnxcu_rmsnorm_launch": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p]),
+    "dnxcu_linear_validate": (C.c_int, [C.POINTER(Linear)]),
+    "dnxcu_linear_pick": (C.c_int, [C.POINTER(Linear)]),
+    "dnxcu_linear_launch": (C.c_int, [C.POINTER(Linear), C.c_void_p]),
+    "dnxcu_linear_plan_create": (C.c_int, [C.POINTER(Linear), C.POINTER(C.c_void_p)]),
+    "dnxcu_linear_plan_launch": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "dnxcu_linear_plan_destroy": (None, [C.c_void_p]),
     "dnxcu_f16_from_float": (C.c_uint16, [C.c_float]),
     "dnxcu_f16_to_float": (C.c_float, [C.c_uint16]),
     "dnxcu_model_create": (C.c_int, [C.POINTER(ModelDesc), C.c_void_p, C.c_int, C.POINTER(C.c_void_p)]),
@@ -280,6 +296,38 @@ def rmsnorm_desc(rows, channels, x, out, out_dtype=DT_F16, eps=1e-5, residual=No
 def rmsnorm(desc: RmsNorm, stream: int = 0):
     """Enqueues the norm on `stream`."""
     check(L.dnxcu_rmsnorm_launch(desc, stream), "dnxcu_rmsnorm_launch")
+
+
+def linear_desc(rows, c_in, c_out, x, weights, out, dtype=DT_F16, activation=ACT_NONE, leaky_alpha=0.0, x_scale=None,
+                w_scale=None, bias=None, residual=None, x_stride=0, w_stride=0, residual_stride=0, out_stride=0,
+                variant=LINEAR_AUTO, device_status=None) -> Linear:
+    """Record of a linear layer (device pointers as integers; strides in elements, 0 = packed rows)."""
+    return Linear(rows, c_in, c_out, dtype, activation, leaky_alpha, variant, x, x_stride, weights, w_stride, x_scale,
+                  w_scale, bias, residual, residual_stride, out, out_stride, device_status)
+
+
+def linear(desc: Linear, stream: int = 0):
+    """Enqueues the layer on `stream`."""
+    check(L.dnxcu_linear_launch(desc, stream), "dnxcu_linear_launch")
+
+
+class LinearPlan:
+    """A linear layer on fixed buffers, planned once and launched many times."""
+
+    def __init__(self, desc: Linear):
+        self._h = C.c_void_p()
+        check(L.dnxcu_linear_plan_create(desc, C.byref(self._h)), "dnxcu_linear_plan_create")
+
+    def launch(self, stream: int = 0):
+        check(L.dnxcu_linear_plan_launch(self._h, stream), "dnxcu_linear_plan_launch")
+
+    def close(self):
+        if self._h:
+            L.dnxcu_linear_plan_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        self.close()
 
 
 class Db:

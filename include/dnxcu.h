@@ -312,6 +312,58 @@ typedef struct dnxcu_rmsnorm {
 DNXCU_API int dnxcu_rmsnorm_validate(const dnxcu_rmsnorm *d);
 DNXCU_API int dnxcu_rmsnorm_launch(const dnxcu_rmsnorm *d, void *stream);
 
+/* Linear layer (matrix product with bias, activation and residual in its epilogue), also the 1x1 convolution of an
+ * HWC tensor:
+ *   s             = x_scale[m] * w_scale[n] * sum_k x[m][k] * weights[n][k]       (a scale of 1 where none is given)
+ *   out[m][n]     = residual[m][n] + activation(s + bias[n])                      rounded once, to binary16
+ * x and weights are both binary16 or both e4m3; weights keep the row-major [c_out][c_in] order they are trained in
+ * (no re-layout).  Products are summed in 32 bits; bias, activation and residual are applied in 32 bits.  NaN and
+ * infinities go the way of the formula; an activation of a NaN is NaN.
+ * out may be residual itself (same pointer and stride) and overlaps nothing else. */
+typedef enum dnxcu_linear_variant {
+  DNXCU_LINEAR_AUTO = 0,  /* picked by sizes, type and alignment */
+  DNXCU_LINEAR_ROWS = 1,  /* at most 16 rows: weights streamed past the rows' registers; x and weights on 16 byte
+                             boundaries, row strides and c_in multiples of 16 bytes */
+  DNXCU_LINEAR_SPLIT = 2, /* few rows on the tensor cores: c_in split over the blocks of a cluster; x and weights on 16
+                             byte boundaries with row strides that are multiples of 16 bytes */
+  DNXCU_LINEAR_TILE = 3,  /* tiles of rows on the tensor cores; x and weights as for SPLIT */
+  DNXCU_LINEAR_ANY = 4    /* the tile kernel with operands fetched by plain loads: any alignment, any stride */
+} dnxcu_linear_variant;
+
+typedef struct dnxcu_linear {
+  int64_t rows;
+  int32_t c_in, c_out;
+  int32_t dtype;       /* dnxcu_dtype of x and weights */
+  int32_t activation;  /* dnxcu_activation */
+  float leaky_alpha;   /* slope of DNXCU_ACT_LEAKY */
+  int32_t variant;     /* dnxcu_linear_variant */
+  const void *x;       /* [rows][c_in] */
+  int64_t x_stride;
+  const void *weights; /* [c_out][c_in] */
+  int64_t w_stride;
+  const float *x_scale;  /* [rows] or NULL */
+  const float *w_scale;  /* [c_out] or NULL */
+  const void *bias;      /* binary16 [c_out] or NULL */
+  const void *residual;  /* binary16 [rows][c_out] or NULL */
+  int64_t residual_stride;
+  void *out;             /* binary16 [rows][c_out] */
+  int64_t out_stride;
+  int32_t *device_status; /* optional device int, see dnxcu_dispatch: 11 operand stage, 12 stage free,
+                             13 accumulators complete, 14 accumulators free, 15 residual */
+} dnxcu_linear;
+
+DNXCU_API int dnxcu_linear_validate(const dnxcu_linear *d);
+/* The variant that AUTO picks (or the forced one); a negative status when the record cannot run. */
+DNXCU_API int dnxcu_linear_pick(const dnxcu_linear *d);
+DNXCU_API int dnxcu_linear_launch(const dnxcu_linear *d, void *stream);
+/* The same planned once and launched many times, as dnxcu_plan_create does for a dispatch: checks, geometry and tensor
+ * maps are worked out when the plan is made, on the device that is current then; launching it with another device
+ * current is DNXCU_E_STATE.  A plan holds no device memory and may be launched on several streams. */
+typedef struct dnxcu_linear_plan dnxcu_linear_plan;
+DNXCU_API int dnxcu_linear_plan_create(const dnxcu_linear *d, dnxcu_linear_plan **out);
+DNXCU_API int dnxcu_linear_plan_launch(const dnxcu_linear_plan *p, void *stream);
+DNXCU_API void dnxcu_linear_plan_destroy(dnxcu_linear_plan *p);
+
 /* float -> binary16 exactly as the reference converts fp32 model weights:
  * mantissa truncated, sub-normal results flushed to zero
  * (common/src/denox/memory/dtype/f16.cpp:6-20). */

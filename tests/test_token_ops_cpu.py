@@ -48,3 +48,73 @@ def test_rmsnorm_limits(kw):
 def test_rmsnorm_overlap(kw):
     """An output that shares bytes with another operand, other than exactly in place."""
     assert norm(**kw) == lib.E_BAD_ARG
+
+
+XS, WS = 0x70000000, 0x80000000
+ST = 0x90000000
+
+
+def linear(**kw):
+    a = dict(rows=40, c_in=64, c_out=96, x=X, weights=W, out=O, residual=R, bias=S, x_scale=XS, w_scale=WS)
+    a.update(kw)
+    return lib.linear_desc(**a)
+
+
+def test_linear_accepts_and_picks():
+    def pick(**kw):
+        d = linear(**kw)
+        st = lib.L.dnxcu_linear_validate(d)
+        got = lib.L.dnxcu_linear_pick(d)
+        assert (st == lib.OK) == (got > 0) and (st == lib.OK or st == got)
+        return got
+
+    assert pick(rows=1) == lib.LINEAR_ROWS
+    assert pick(rows=100) == lib.LINEAR_SPLIT
+    assert pick(rows=100000) == lib.LINEAR_TILE
+    assert pick(rows=100000, dtype=lib.DT_E4M3) == lib.LINEAR_TILE
+    assert pick(c_in=65) == lib.LINEAR_ANY and pick(x=X + 2) == lib.LINEAR_ANY and pick(weights=W + 8) == lib.LINEAR_ANY
+    assert pick(c_in=65, x_stride=72, w_stride=80) != lib.LINEAR_ANY  # padded rows
+    assert pick(dtype=lib.DT_E4M3, c_in=72) == lib.LINEAR_ANY
+    assert pick(residual=None, bias=None, x_scale=None, w_scale=None, rows=1, c_in=1, c_out=1) == lib.LINEAR_ANY
+    assert pick(residual=O) > 0  # in place
+    for v, kw in ((lib.LINEAR_ROWS, dict(rows=16)), (lib.LINEAR_SPLIT, {}), (lib.LINEAR_TILE, {}), (lib.LINEAR_ANY, {})):
+        assert pick(variant=v, **kw) == v
+    for v, kw in ((lib.LINEAR_ROWS, dict(rows=17)), (lib.LINEAR_ROWS, dict(rows=4, c_in=68, x_stride=72, w_stride=72)),
+                  (lib.LINEAR_SPLIT, dict(x=X + 2)), (lib.LINEAR_TILE, dict(c_in=65))):
+        assert pick(variant=v, **kw) == lib.E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(rows=0), dict(c_in=0), dict(c_out=-5), dict(x=None), dict(weights=None), dict(out=None),
+                                dict(dtype=2), dict(dtype=-1), dict(activation=6), dict(activation=-1), dict(variant=5),
+                                dict(x_stride=63), dict(w_stride=1), dict(out_stride=95), dict(residual_stride=-96)])
+def test_linear_bad_arguments(kw):
+    assert lib.L.dnxcu_linear_validate(linear(**kw)) == lib.E_BAD_ARG
+
+
+@pytest.mark.parametrize("kw", [dict(x=X + 1), dict(weights=W + 1), dict(out=O + 1), dict(residual=R + 1), dict(bias=S + 1),
+                                dict(x_scale=XS + 2), dict(w_scale=WS + 1), dict(device_status=ST + 1)])
+def test_linear_misaligned(kw):
+    assert lib.L.dnxcu_linear_validate(linear(**kw)) == lib.E_MISALIGNED
+
+
+@pytest.mark.parametrize("kw", [dict(rows=1 << 31), dict(c_in=(1 << 24) + 1), dict(c_out=(1 << 24) + 1), dict(x_stride=1 << 35),
+                                dict(out_stride=1 << 35)])
+def test_linear_limits(kw):
+    assert lib.L.dnxcu_linear_validate(linear(**kw)) == lib.E_LIMIT
+
+
+@pytest.mark.parametrize("kw", [dict(out=X), dict(out=W), dict(out=R + 2), dict(residual=O, residual_stride=128), dict(bias=O),
+                                dict(x_scale=O + 4), dict(w_scale=O), dict(device_status=O), dict(out=X + 64 * 39 * 2)])
+def test_linear_overlap(kw):
+    assert lib.L.dnxcu_linear_validate(linear(**kw)) == lib.E_BAD_ARG
+
+
+def test_null_records():
+    import ctypes as C
+    p = C.c_void_p()
+    assert lib.L.dnxcu_linear_validate(None) == lib.E_BAD_ARG and lib.L.dnxcu_linear_launch(None, None) == lib.E_BAD_ARG
+    assert lib.L.dnxcu_linear_plan_create(None, C.byref(p)) == lib.E_BAD_ARG
+    assert lib.L.dnxcu_linear_plan_create(linear(), None) == lib.E_BAD_ARG
+    assert lib.L.dnxcu_linear_plan_launch(None, None) == lib.E_BAD_ARG
+    assert lib.L.dnxcu_rmsnorm_validate(None) == lib.E_BAD_ARG and lib.L.dnxcu_rmsnorm_launch(None, None) == lib.E_BAD_ARG
+    lib.L.dnxcu_linear_plan_destroy(None)
