@@ -17,7 +17,6 @@
 //   block form rows up to 32 elements x 1024 threads: a block per row;
 //   loop form  anything longer (or long and unaligned): a block per row that reads it twice, the second time from L2.
 #include "internal.h"
-#include <cuda_fp8.h>
 #include <math.h>
 
 namespace dnxcu {
@@ -49,16 +48,30 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 
 // Loads of data that an output of the same call may alias are plain loads (never the read-only path); every thread
 // reads an element before it writes it, and no thread reads another's.
-template <int V>
-__device__ __forceinline__ void load_sum(const NormArgs &g, long long row, int c, float (&h)[V]) {
-  Halves<V> a;
-  a.v = *reinterpret_cast<const typename Vec<V>::H *>(g.x + row * g.xs + c);
+// Raw first, all of a thread's loads before the first conversion: that is what keeps them in flight together.
+template <int V, bool RES>
+struct Raw {
+  typename Vec<V>::H x, r;
+};
+template <int V, bool RES>
+__device__ __forceinline__ void load_raw(const NormArgs &g, long long row, int c, bool in, Raw<V, RES> &a) {
+  a.x = typename Vec<V>::H();
+  if (RES) a.r = typename Vec<V>::H();
+  if (in) {
+    a.x = *reinterpret_cast<const typename Vec<V>::H *>(g.x + row * g.xs + c);
+    if (RES) a.r = *reinterpret_cast<const typename Vec<V>::H *>(g.residual + row * g.rs + c);
+  }
+}
+template <int V, bool RES>
+__device__ __forceinline__ void sum_raw(const Raw<V, RES> &a, float (&h)[V]) {
+  Halves<V> t;
+  t.v = a.x;
 #pragma unroll
-  for (int e = 0; e < V; ++e) h[e] = __half2float(a.h[e]);
-  if (g.residual) {
-    a.v = *reinterpret_cast<const typename Vec<V>::H *>(g.residual + row * g.rs + c);
+  for (int e = 0; e < V; ++e) h[e] = __half2float(t.h[e]);
+  if (RES) {
+    t.v = a.r;
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] += __half2float(a.h[e]);
+    for (int e = 0; e < V; ++e) h[e] += __half2float(t.h[e]);
   }
 }
 template <int V>
@@ -73,31 +86,56 @@ __device__ __forceinline__ void load_weight(const NormArgs &g, int c, float (&w)
     for (int e = 0; e < V; ++e) w[e] = 1.0f;
   }
 }
+// Two values to binary16 or e4m3 at once.  The packed conversions run on the wide pipes; single ones go through the
+// transcendental unit, a fraction as wide.
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint16_t pack_e4m3(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <int V>
+__device__ __forceinline__ void store_halves(__half *p, const float (&y)[V]) {
+  union {
+    typename Vec<V>::H v;
+    uint32_t w[(V + 1) / 2];
+  } a;
+  if constexpr (V == 1) {
+    *reinterpret_cast<uint16_t *>(p) = (uint16_t)pack_f16(y[0], 0.0f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) a.w[e / 2] = pack_f16(y[e], y[e + 1]);
+    *reinterpret_cast<typename Vec<V>::H *>(p) = a.v;
+  }
+}
 template <int V>
 __device__ __forceinline__ void store_sum(const NormArgs &g, long long row, int c, const float (&h)[V]) {
-  Halves<V> a;
-#pragma unroll
-  for (int e = 0; e < V; ++e) a.h[e] = __float2half_rn(h[e]);
-  *reinterpret_cast<typename Vec<V>::H *>(g.sum + row * g.ss + c) = a.v;
+  store_halves<V>(g.sum + row * g.ss + c, h);
 }
 // y = weight * h * f, rounded once to the output type.  8 bits: f = 448 / max|weight * h|; a product that the last
 // bit of f puts above 448 saturates to it.
 template <int V, bool Q>
 __device__ __forceinline__ void store_out(const NormArgs &g, long long row, int c, const float (&h)[V], const float (&w)[V],
                                           float f) {
-  if (Q) {
+  float y[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) y[e] = Q ? h[e] * w[e] * f : h[e] * f * w[e];
+  if constexpr (!Q) {
+    store_halves<V>((__half *)g.out + row * g.os + c, y);
+  } else if constexpr (V == 1) {
+    ((uint8_t *)g.out)[row * g.os + c] = (uint8_t)pack_e4m3(y[0], 0.0f);
+  } else {
     union {
       typename Vec<V>::Q v;
-      uint8_t b[V];
+      uint16_t w[V / 2];
     } q;
 #pragma unroll
-    for (int e = 0; e < V; ++e) q.b[e] = __nv_cvt_float_to_fp8(h[e] * w[e] * f, __NV_SATFINITE, __NV_E4M3);
+    for (int e = 0; e < V; e += 2) q.w[e / 2] = pack_e4m3(y[e], y[e + 1]);
     *reinterpret_cast<typename Vec<V>::Q *>((uint8_t *)g.out + row * g.os + c) = q.v;
-  } else {
-    Halves<V> a;
-#pragma unroll
-    for (int e = 0; e < V; ++e) a.h[e] = __float2half_rn(h[e] * f * w[e]);
-    *reinterpret_cast<typename Vec<V>::H *>((__half *)g.out + row * g.os + c) = a.v;
   }
 }
 // The row's factor from its statistics; `top` = bits of max|weight * h|.
@@ -119,7 +157,7 @@ __device__ __forceinline__ float row_factor(const NormArgs &g, float ss, uint32_
 
 // ---- warp form --------------------------------------------------------------
 // 2^LT lanes per row; a thread holds vectors t, t + 2^LT, ... of U rows.
-template <int V, int E, bool Q>
+template <int V, int E, bool Q, bool RES>
 __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
   constexpr int N = E / V, U = 32 / E;
   const int tpr = 1 << lt, t = threadIdx.x & (tpr - 1);
@@ -127,7 +165,7 @@ __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
   const long long rows_per_block = (long long)per_block * U;
   const int nv = g.C / V;
   for (long long r0 = (long long)blockIdx.x * rows_per_block; r0 < g.rows; r0 += (long long)gridDim.x * rows_per_block) {
-    float h[U][N][V];
+    Raw<V, RES> raw[U][N];
     long long row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -135,12 +173,7 @@ __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int vi = t + (i << lt);
-        if (row[u] < g.rows && vi < nv) {
-          load_sum<V>(g, row[u], vi * V, h[u][i]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) h[u][i][e] = 0.0f;
-        }
+        load_raw<V, RES>(g, row[u], vi * V, row[u] < g.rows && vi < nv, raw[u][i]);
       }
     }
     float w[N][V];
@@ -154,15 +187,17 @@ __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float ss = 0.0f;
+      float h[N][V], ss = 0.0f;
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int i = 0; i < N; ++i) {
+        sum_raw<V, RES>(raw[u][i], h[i]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          ss = fmaf(h[u][i][e], h[u][i][e], ss);
-          if (Q) top = max(top, abs_bits(h[u][i][e] * w[i][e]));
+          ss = fmaf(h[i][e], h[i][e], ss);
+          if (Q) top = max(top, abs_bits(h[i][e] * w[i][e]));
         }
+      }
       for (int o = tpr >> 1; o > 0; o >>= 1) {
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (Q) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -175,8 +210,8 @@ __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
       for (int i = 0; i < N; ++i) {
         const int vi = t + (i << lt);
         if (vi < nv) {
-          if (g.sum) store_sum<V>(g, row[u], vi * V, h[u][i]);
-          store_out<V, Q>(g, row[u], vi * V, h[u][i], w[i], f);
+          if (g.sum) store_sum<V>(g, row[u], vi * V, h[i]);
+          store_out<V, Q>(g, row[u], vi * V, h[i], w[i], f);
         }
       }
     }
@@ -205,23 +240,18 @@ __device__ __forceinline__ void block_reduce(float &ss, uint32_t &top, int turn)
 }
 
 // ---- block form -------------------------------------------------------------
-template <int V, int E, bool Q>
+template <int V, int E, bool Q, bool RES>
 __global__ void __launch_bounds__(1024) rmsnorm_block(NormArgs g) {
   constexpr int N = E / V;
   const int nv = g.C / V, t = threadIdx.x, nt = blockDim.x;
   int turn = 0;
   for (long long row = blockIdx.x; row < g.rows; row += gridDim.x, turn ^= 1) {
+    Raw<V, RES> raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) load_raw<V, RES>(g, row, (t + i * nt) * V, t + i * nt < nv, raw[i]);
     float h[N][V];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int vi = t + i * nt;
-      if (vi < nv) {
-        load_sum<V>(g, row, vi * V, h[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) h[i][e] = 0.0f;
-      }
-    }
+    for (int i = 0; i < N; ++i) sum_raw<V, RES>(raw[i], h[i]);
     float ss = 0.0f;
     uint32_t top = 0;
 #pragma unroll
@@ -253,7 +283,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_block(NormArgs g) {
 }
 
 // ---- loop form --------------------------------------------------------------
-template <int V, bool Q>
+template <int V, bool Q, bool RES>
 __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
   const int nv = g.C / V, t = threadIdx.x, nt = blockDim.x;
   int turn = 0;
@@ -263,7 +293,9 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
 #pragma unroll 4
     for (int vi = t; vi < nv; vi += nt) {
       float h[V], w[V];
-      load_sum<V>(g, row, vi * V, h);
+      Raw<V, RES> raw;
+      load_raw<V, RES>(g, row, vi * V, true, raw);
+      sum_raw<V, RES>(raw, h);
       if (Q) load_weight<V>(g, vi * V, w);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -278,7 +310,9 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
 #pragma unroll 4
     for (int vi = t; vi < nv; vi += nt) {
       float h[V], w[V];
-      load_sum<V>(g, row, vi * V, h);
+      Raw<V, RES> raw;
+      load_raw<V, RES>(g, row, vi * V, true, raw);
+      sum_raw<V, RES>(raw, h);
       load_weight<V>(g, vi * V, w);
       if (g.sum) store_sum<V>(g, row, vi * V, h);
       store_out<V, Q>(g, row, vi * V, h, w, f);
@@ -288,7 +322,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
 
 constexpr unsigned kMaxGrid = 0x7fffffffu;
 
-template <int V, bool Q>
+template <int V, bool Q, bool RES>
 void launch_v(const NormArgs &g, cudaStream_t s) {
   const int nv = g.C / V;
   if (g.C <= 1024) {
@@ -299,9 +333,9 @@ void launch_v(const NormArgs &g, cudaStream_t s) {
     const long long per_block = (256 >> lt) * (32 / e);
     const long long blocks = (g.rows + per_block - 1) / per_block;
     const unsigned grid = (unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid);
-    if (e == 8) rmsnorm_warp<V, 8, Q><<<grid, 256, 0, s>>>(g, lt);
-    else if (e == 16) rmsnorm_warp<V, 16, Q><<<grid, 256, 0, s>>>(g, lt);
-    else rmsnorm_warp<V, 32, Q><<<grid, 256, 0, s>>>(g, lt);
+    if (e == 8) rmsnorm_warp<V, 8, Q, RES><<<grid, 256, 0, s>>>(g, lt);
+    else if (e == 16) rmsnorm_warp<V, 16, Q, RES><<<grid, 256, 0, s>>>(g, lt);
+    else rmsnorm_warp<V, 32, Q, RES><<<grid, 256, 0, s>>>(g, lt);
     return;
   }
   const unsigned grid = (unsigned)(g.rows < kMaxGrid ? g.rows : kMaxGrid);
@@ -310,16 +344,18 @@ void launch_v(const NormArgs &g, cudaStream_t s) {
     return (t + 31) / 32 * 32;
   };
   // few rows: as many threads per row as there are, for latency; many rows: 32 elements in flight per thread
-  if (g.rows <= 148 && threads(8) <= 1024) rmsnorm_block<V, 8, Q><<<grid, threads(8), 0, s>>>(g);
-  else if (g.rows <= 148 && threads(16) <= 1024) rmsnorm_block<V, 16, Q><<<grid, threads(16), 0, s>>>(g);
-  else if (threads(32) <= 1024) rmsnorm_block<V, 32, Q><<<grid, threads(32), 0, s>>>(g);
-  else rmsnorm_loop<V, Q><<<grid, 1024, 0, s>>>(g);
+  if (g.rows <= 148 && threads(8) <= 1024) rmsnorm_block<V, 8, Q, RES><<<grid, threads(8), 0, s>>>(g);
+  else if (g.rows <= 148 && threads(16) <= 1024) rmsnorm_block<V, 16, Q, RES><<<grid, threads(16), 0, s>>>(g);
+  else if (threads(32) <= 1024) rmsnorm_block<V, 32, Q, RES><<<grid, threads(32), 0, s>>>(g);
+  else rmsnorm_loop<V, Q, RES><<<grid, 1024, 0, s>>>(g);
 }
 
 template <int V>
 void launch_q(const NormArgs &g, bool q, cudaStream_t s) {
-  if (q) launch_v<V, true>(g, s);
-  else launch_v<V, false>(g, s);
+  if (q && g.residual) launch_v<V, true, true>(g, s);
+  else if (q) launch_v<V, true, false>(g, s);
+  else if (g.residual) launch_v<V, false, true>(g, s);
+  else launch_v<V, false, false>(g, s);
 }
 
 // The record with packed strides filled in, or why it cannot run.

@@ -327,7 +327,8 @@ class LinearPlan:
             self._h = C.c_void_p()
 
     def __del__(self):
-        self.close()
+        if L is not None:  # (interpreter shutdown)
+            self.close()
 
 
 class Db:
