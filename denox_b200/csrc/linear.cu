@@ -35,6 +35,11 @@ struct LinArgs {
   int kb;        // 128 byte wide steps along c_in
   int stages;
   int split;     // split: blocks per cluster
+  int overlay;   // split: the received partial sums lie over the operand stages
+  int teams;     // tile: epilogue teams
+  int bufs;      // tile: accumulators
+  int w_res;     // tile: the weights of the (one) column of tiles stay in shared memory
+  int group;     // tile: tiles along the rows that are walked together
   int out_tma, res_tma;
   int *status;
   unsigned long long wait_limit;
@@ -182,9 +187,10 @@ __device__ __forceinline__ int k_steps(const LinArgs &g, int kb) {
   return bytes >= 128 ? 4 : (bytes + 31) / 32;
 }
 
-constexpr int MAX_STAGES = 8;
-constexpr int HDR_FULL = 0, HDR_EMPTY = 8 * MAX_STAGES, HDR_TFULL = 16 * MAX_STAGES, HDR_TEMPTY = HDR_TFULL + 16,
-              HDR_RES = HDR_TEMPTY + 16, HDR_TMEM = HDR_RES + 64, HDR_ABORT = HDR_TMEM + 4;
+constexpr int MAX_STAGES = 12;
+constexpr int MAX_BUFS = 4;  // accumulators in tensor memory
+constexpr int HDR_FULL = 0, HDR_EMPTY = 8 * MAX_STAGES, HDR_TFULL = 16 * MAX_STAGES, HDR_TEMPTY = HDR_TFULL + 8 * MAX_BUFS,
+              HDR_RES = HDR_TEMPTY + 8 * MAX_BUFS, HDR_WRES = HDR_RES + 64, HDR_TMEM = HDR_WRES + 8, HDR_ABORT = HDR_TMEM + 4;
 static_assert((HDR_ABORT + 4) % 8 == 0 && HDR_ABORT + 12 <= 1024, "header layout");
 constexpr int HEADER = 1024;
 constexpr uint32_t kSmemLimit = 232448;
@@ -192,10 +198,12 @@ constexpr uint32_t kSmemLimit = 232448;
 __device__ __forceinline__ uint32_t aligned_base(const void *dyn) { return (smem_u32(dyn) + 1023u) & ~1023u; }
 
 // ---- TILE and ANY -----------------------------------------------------------
-// 12 warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7 and 8-11 are two epilogue teams that
-// take alternate tiles; each team has one of the two accumulators, so one tile is multiplied while the teams finish the
-// ones before.  ANY: warps 8-11 fetch instead, one team takes both accumulators.
-constexpr int TILE_THREADS = 384;
+// Warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7 and 8-11 are two epilogue teams that take
+// alternate tiles (or one team takes all); 2 or 4 accumulators rotate, so tiles are multiplied while the teams finish the
+// ones before.  ANY: warps 12-15 fetch with plain loads instead, each a whole stage, so four stages are on their way at
+// any time.  Where all of c_out is one column of tiles and the weights are small (a pointwise layer over pixels), they are
+// fetched once per block and only rows of x stream.
+constexpr int TILE_THREADS = 384, ANY_THREADS = 512;
 constexpr int COLBUF = 512;              // per epilogue warp: bias and weight scale of 64 channels
 constexpr int TILE_FIXED = HEADER + 8 * COLBUF;
 constexpr int STAGING = 4096;            // per epilogue warp: 32 rows x 64 channels of binary16
@@ -203,68 +211,115 @@ constexpr int STAGING = 4096;            // per epilogue warp: 32 rows x 64 chan
 struct TilePos {
   int m, n;
 };
-// Tiles in groups of `G` along the rows, so that the tiles in flight share operands in L2.
-__device__ __forceinline__ TilePos tile_pos(const LinArgs &g, int t, int G) {
+// Tiles in groups of `group` along the rows, so that the tiles in flight share operands in L2.
+__device__ __forceinline__ TilePos tile_pos(const LinArgs &g, int t) {
   if (g.nt == 1) return {t, 0};
-  const int per = G * g.nt, grp = t / per, r = t - grp * per;
-  const int m0 = grp * G, gm = min(G, g.mt - m0);
+  const int per = g.group * g.nt, grp = t / per, r = t - grp * per;
+  const int m0 = grp * g.group, gm = min(g.group, g.mt - m0);
   const int n = r / gm;
   return {m0 + r - n * gm, n};
 }
 
-// 8 elements (16 bytes) or 16 e4m3 of one operand row from channel byte `kbyte` on, zero beyond the row: plain loads.
+// 16 bytes of an operand row at any alignment, zero beyond the row's end.  `begin` and `end` bound the whole operand: the
+// aligned 16 byte words around the piece are read where they lie inside it (between rows there are bytes of the same
+// buffer) and shifted together; at the operand's two ends single elements are read instead.
+struct PieceReq {
+  uint4 a, b;
+  const uint8_t *p;
+  int left;
+  bool slow;
+};
+__device__ __forceinline__ void request_piece(PieceReq &q, const uint8_t *row, int kbyte, int kbytes, const uint8_t *begin,
+                                              const uint8_t *end) {
+  q.left = row ? kbytes - kbyte : 0;
+  q.p = row + kbyte;
+  q.a = q.b = make_uint4(0, 0, 0, 0);
+  q.slow = false;
+  if (q.left <= 0) return;
+  const int sh = (int)((uintptr_t)q.p & 15), need = sh + (q.left < 16 ? q.left : 16);
+  const uint8_t *w = q.p - sh;
+  q.slow = w < begin || w + (need > 16 ? 32 : 16) > end;
+  if (q.slow) return;
+  q.a = __ldg(reinterpret_cast<const uint4 *>(w));
+  if (need > 16) q.b = __ldg(reinterpret_cast<const uint4 *>(w + 16));
+}
 template <bool F8>
-__device__ __forceinline__ uint4 fetch_piece(const uint8_t *row, int kbyte, int kbytes) {
-  const int left = kbytes - kbyte;
-  if (left <= 0) return make_uint4(0, 0, 0, 0);
-  const uint8_t *p = row + kbyte;
-  if (left >= 16 && ((uintptr_t)p & 15) == 0) return __ldg(reinterpret_cast<const uint4 *>(p));
-  uint32_t w[4];
-  if (F8) {
+__device__ __forceinline__ uint4 finish_piece(const PieceReq &q) {
+  uint32_t w[8] = {q.a.x, q.a.y, q.a.z, q.a.w, q.b.x, q.b.y, q.b.z, q.b.w};
+  if (q.slow) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       w[i] = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i * 4 + e < left) w[i] |= (uint32_t)__ldg(p + i * 4 + e) << (8 * e);
+      for (int e = 0; e < (F8 ? 4 : 2); ++e) {
+        const int at = i * 4 + e * (F8 ? 1 : 2);
+        if (at < q.left)
+          w[i] |= (F8 ? (uint32_t)__ldg(q.p + at) : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(q.p + at))) << (at % 4 * 8);
+      }
     }
-  } else {
-    const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  const int sh = (int)((uintptr_t)q.p & 15);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = 0;
+  for (int i = 0; i < 6; ++i) w[i] = sh & 8 ? w[i + 2] : w[i];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (i * 4 + e * 2 < left) w[i] |= (uint32_t)__ldg(q + i * 2 + e) << (16 * e);
+  for (int i = 0; i < 5; ++i) w[i] = sh & 4 ? w[i + 1] : w[i];
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = __funnelshift_r(w[i], w[i + 1], (sh & 3) * 8);
+    const int keep = q.left - i * 4;  // bytes of this word that lie inside the row
+    if (keep < 4) o[i] = keep <= 0 ? 0u : o[i] & (0xffffffffu >> (32 - 8 * keep));
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// One warp fills `rows` rows (from row `row0` of an operand of `n` rows) of a swizzled tile with `pieces` pieces each.
+template <bool F8>
+__device__ __forceinline__ void fill_tile(uint32_t dst, const uint8_t *op, long long stride, long long row0, int n, int rows,
+                                          int pieces, int kb, int kbytes, int lane, int first, int step) {
+  const uint8_t *end = op + (long long)(n - 1) * stride + kbytes;
+  const int items = rows * pieces;
+  constexpr int B = 4;
+  for (int i0 = first * 32 + lane; i0 < items; i0 += 32 * step * B) {
+    PieceReq q[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int i = i0 + 32 * step * u, r = i / pieces, j = i - r * pieces;
+      request_piece(q[u], i < items && row0 + r < n ? op + (row0 + r) * stride : nullptr, kb * 128 + j * 16, kbytes, op, end);
+    }
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int i = i0 + 32 * step * u, r = i / pieces, j = i - r * pieces;
+      const uint4 v = finish_piece<F8>(q[u]);
+      if (i < items) sts128(dst + (uint32_t)r * 128u + (uint32_t)((j ^ (r & 7)) << 4), v);
     }
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int CG, bool F8, bool ANY>
-__global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
+__global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
   extern __shared__ uint8_t dyn[];
   const uint32_t base = aligned_base(dyn);
   uint8_t *hdr = dyn + (base - smem_u32(dyn));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(hdr + HDR_ABORT);
-  const uint32_t b_rows = (uint32_t)g.BN / CG;
-  const uint32_t stage_bytes = 16384u + b_rows * 128u;
-  const uint32_t stage0 = base + TILE_FIXED, staging0 = stage0 + stage_bytes * (uint32_t)g.stages;
+  const uint32_t b_rows = (uint32_t)g.BN / CG, b_bytes = b_rows * 128u;
+  const uint32_t stage_bytes = 16384u + (g.w_res ? 0u : b_bytes);
+  const uint32_t wres0 = base + TILE_FIXED, stage0 = wres0 + (g.w_res ? (uint32_t)g.kb * b_bytes : 0u);
+  const uint32_t staging0 = stage0 + stage_bytes * (uint32_t)g.stages;
   const int ntiles = g.mt * g.nt, step = (int)gridDim.x / CG, first = (int)blockIdx.x / CG;
-  constexpr int GROUP = CG == 2 ? 8 : 16;
-  constexpr int TEAMS = ANY ? 1 : 2;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     *reinterpret_cast<volatile unsigned long long *>(abort_flag + 1) = g.wait_limit;
     for (int i = 0; i < MAX_STAGES; ++i) {
-      mbar_init(base + HDR_FULL + 8 * i, ANY ? 4 : 1);
+      mbar_init(base + HDR_FULL + 8 * i, 1);
       mbar_init(base + HDR_EMPTY + 8 * i, 1);
-      mbar_init(base + HDR_RES + 8 * i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 8; ++i) mbar_init(base + HDR_RES + 8 * i, 1);
+    mbar_init(base + HDR_WRES, ANY ? 4 : 1);
+    for (int i = 0; i < MAX_BUFS; ++i) {
       mbar_init(base + HDR_TFULL + 8 * i, 1);
       mbar_init(base + HDR_TEMPTY + 8 * i, 4 * CG);
     }
@@ -287,11 +342,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
   if (!ANY && warp == 0) {
     // ---- operand tiles by TMA; the pair's bytes are counted on the first block's barrier ----
     if (lane == 0) {
+      if (g.w_res) {
+        mbar_expect_tx(base + HDR_WRES, (uint32_t)g.kb * b_bytes);
+        for (int kb = 0; kb < g.kb; ++kb)
+          tma_load_2d<1>(wres0 + (uint32_t)kb * b_bytes, &g.tm_w, kb * (F8 ? 128 : 64), 0, base + HDR_WRES);
+      }
       int s = 0;
       uint32_t ph = 1;
       bool ok = true;
       for (int t = first; ok && t < ntiles; t += step) {
-        const TilePos p = tile_pos(g, t, GROUP);
+        const TilePos p = tile_pos(g, t);
         const int row_a = p.m * (128 * CG) + (int)rank * 128, row_b = p.n * g.BN + (int)(rank * b_rows);
         for (int kb = 0; kb < g.kb; ++kb) {
           ok = mbar_wait(base + HDR_EMPTY + 8 * s, ph, abort_flag, g.status, 12);
@@ -301,7 +361,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
           const uint32_t bar = CG == 2 ? map_rank(full, 0) : full;
           const uint32_t a = stage0 + stage_bytes * (uint32_t)s;
           tma_load_2d<CG>(a, &g.tm_x, kb * (F8 ? 128 : 64), row_a, bar);
-          tma_load_2d<CG>(a + 16384u, &g.tm_w, kb * (F8 ? 128 : 64), row_b, bar);
+          if (!g.w_res) tma_load_2d<CG>(a + 16384u, &g.tm_w, kb * (F8 ? 128 : 64), row_b, bar);
           if (++s == g.stages) {
             s = 0;
             ph ^= 1;
@@ -309,36 +369,36 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
         }
       }
     }
-  } else if (ANY && warp >= 8) {
+  } else if (ANY && warp >= 12) {
     // ---- operand tiles by plain loads, swizzled as the copy engine would ----
-    const int tid = threadIdx.x - 256;
+    const int pw = warp - 12;
     const int kbytes = F8 ? g.K : 2 * g.K;
-    int s = 0;
+    if (g.w_res) {
+      for (int kb = 0; kb < g.kb; ++kb)
+        fill_tile<F8>(wres0 + (uint32_t)kb * b_bytes, g.w, g.ws, 0, g.N, g.BN, 2 * k_steps<F8>(g, kb), kb, kbytes, lane, pw, 4);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(base + HDR_WRES);
+    }
+    int s = 0, turn = 0;
     uint32_t ph = 1;
     bool ok = true;
     for (int t = first; ok && t < ntiles; t += step) {
-      const TilePos p = tile_pos(g, t, GROUP);
+      const TilePos p = tile_pos(g, t);
       for (int kb = 0; kb < g.kb; ++kb) {
-        ok = mbar_wait(base + HDR_EMPTY + 8 * s, ph, abort_flag, g.status, 12);
-        ok = __all_sync(0xffffffffu, ok);  // (the warp leaves the loop as one)
-        if (!ok) break;
-        const uint32_t a = stage0 + stage_bytes * (uint32_t)s;
-        const int pieces = 2 * k_steps<F8>(g, kb);  // 16 byte pieces of a row that the MMAs will read
-        const int items = (128 + g.BN) * pieces;
-#pragma unroll 4
-        for (int i = tid; i < items; i += 128) {
-          const int r = i / pieces, j = i - r * pieces;
-          const bool is_w = r >= 128;
-          const int rr = is_w ? r - 128 : r;
-          const long long row = is_w ? (long long)p.n * g.BN + rr : (long long)p.m * 128 + rr;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (row < (is_w ? g.N : g.M))
-            v = fetch_piece<F8>(is_w ? g.w + row * g.ws : g.x + row * g.xs, kb * 128 + j * 16, kbytes);
-          sts128(a + (is_w ? 16384u : 0u) + (uint32_t)rr * 128u + (uint32_t)((j ^ (rr & 7)) << 4), v);
+        if (turn == pw) {
+          ok = mbar_wait(base + HDR_EMPTY + 8 * s, ph, abort_flag, g.status, 12);
+          ok = __all_sync(0xffffffffu, ok);  // (the warp leaves the loop as one)
+          if (!ok) break;
+          const uint32_t a = stage0 + stage_bytes * (uint32_t)s;
+          const int pieces = 2 * k_steps<F8>(g, kb);  // 16 byte pieces of a row that the MMAs will read
+          fill_tile<F8>(a, g.x, g.xs, (long long)p.m * 128, g.M, 128, pieces, kb, kbytes, lane, 0, 1);
+          if (!g.w_res) fill_tile<F8>(a + 16384u, g.w, g.ws, (long long)p.n * g.BN, g.N, g.BN, pieces, kb, kbytes, lane, 0, 1);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(base + HDR_FULL + 8 * s);
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(base + HDR_FULL + 8 * s);
+        turn = (turn + 1) & 3;
         if (++s == g.stages) {
           s = 0;
           ph ^= 1;
@@ -349,20 +409,20 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
     // ---- MMA issue: one thread of the (first) block ----
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = mma_idesc(128 * CG, g.BN);
-      int s = 0, it = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int t = first; ok && t < ntiles; t += step, ++it) {
-        const int buf = it & 1;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, bph = 1;
+      bool ok = !g.w_res || mbar_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
+      for (int t = first; ok && t < ntiles; t += step) {
         const uint32_t d = tmem + (uint32_t)(buf * g.BN);
-        ok = mbar_wait(base + HDR_TEMPTY + 8 * buf, (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, g.status, 14);
+        ok = mbar_wait(base + HDR_TEMPTY + 8 * buf, bph, abort_flag, g.status, 14);
         if (!ok) break;
         tc_fence_after();
         for (int kb = 0; kb < g.kb; ++kb) {
           ok = mbar_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t a = operand_desc(stage0 + stage_bytes * (uint32_t)s), b = a + (16384u >> 4);
+          const uint32_t at = stage0 + stage_bytes * (uint32_t)s;
+          const uint64_t a = operand_desc(at), b = operand_desc(g.w_res ? wres0 + (uint32_t)kb * b_bytes : at + 16384u);
           const int ks = k_steps<F8>(g, kb);
           if (ks == 4) {
 #pragma unroll
@@ -378,9 +438,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
         }
         if (!ok) break;
         mma_commit<CG>(base + HDR_TFULL + 8 * buf);
+        if (++buf == g.bufs) {
+          buf = 0;
+          bph ^= 1;
+        }
       }
     }
-  } else if (warp >= 4 && warp < 4 + 4 * TEAMS) {
+  } else if (warp >= 4 && warp < 4 + 4 * g.teams) {
     // ---- epilogue: 32 rows x 64 channels at a time through a swizzled staging tile ----
     const int ew = warp - 4, team = ew >> 2, q = warp & 3;
     const uint32_t stg = staging0 + (uint32_t)ew * STAGING;
@@ -388,56 +452,73 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
     float *col_b = reinterpret_cast<float *>(hdr + HEADER + ew * COLBUF), *col_s = col_b + 64;
     const uint32_t rbar = base + HDR_RES + 8 * ew;
     const uint32_t my = stg + (uint32_t)lane * 128u;
-    uint32_t rph = 0;
+    const auto staged = [&](int r, int j) {  // channel j of row r in the staging tile
+      return reinterpret_cast<__half *>(stg_p + r * 128 + ((((j >> 3) ^ (r & 7)) << 4) | ((j & 7) << 1)));
+    };
+    uint32_t rph = 0, bph = 0;
     bool ok = true;
-    int it = 0;
+    int it = 0, buf = 0;
     for (int t = first; ok && t < ntiles; t += step, ++it) {
-      if (TEAMS == 2 && (it & 1) != team) continue;
-      const int buf = it & 1;
-      const TilePos p = tile_pos(g, t, GROUP);
+      const int my_buf = buf;
+      const uint32_t my_ph = bph;
+      if (++buf == g.bufs) {
+        buf = 0;
+        bph ^= 1;
+      }
+      if (g.teams == 2 && (it & 1) != team) continue;
+      const TilePos p = tile_pos(g, t);
       const int n0 = p.n * g.BN, nc = min(g.BN, g.N - n0);
       const long long row0 = (long long)p.m * (128 * CG) + (long long)rank * 128 + q * 32, row = row0 + lane;
       const bool live = row0 < g.M;
       const float xs = (g.x_scale && row < g.M) ? __ldg(g.x_scale + row) : 1.0f;
-      const auto fetch_res = [&](int c) {  // (lane 0) the residual's box into the staging tile
-        mbar_expect_tx(rbar, STAGING);
-        tma_load_2d<1>(stg, &g.tm_res, n0 + c, (int)row0, rbar);
-      };
-      if (live && g.res_tma && lane == 0) {
-        bulk_group_wait_read();
-        fetch_res(0);
-      }
-      ok = mbar_wait(base + HDR_TFULL + 8 * buf, (uint32_t)(it >> 1) & 1u, abort_flag, g.status, 13);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t acc = tmem + (uint32_t)(buf * g.BN) + ((uint32_t)(q * 32) << 16);
-      for (int c = 0; live && c < nc; c += 64) {
-        for (int j = lane; j < 64; j += 32) {
-          const int n = n0 + c + j;
+      // What 64 channels need besides the sums: bias, scales and the residual, which goes into the staging tile.
+      const auto prepare = [&](int c) {
+        if (lane == 0) bulk_group_wait_read();  // the staging tile's last store has read it
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = lane + 32 * h, n = n0 + c + j;
           col_b[j] = (g.bias && n < g.N) ? __half2float(__ldg(g.bias + n)) : 0.0f;
           col_s[j] = (g.w_scale && n < g.N) ? __ldg(g.w_scale + n) : 1.0f;
         }
-        if (lane == 0 && (!g.res_tma || c > 0)) {
-          bulk_group_wait_read();  // the staging tile's last store has read it
-          if (g.res_tma) fetch_res(c);
-        }
         __syncwarp();
+        if (g.res_tma) {
+          if (lane == 0) {
+            mbar_expect_tx(rbar, STAGING);
+            tma_load_2d<1>(stg, &g.tm_res, n0 + c, (int)row0, rbar);
+          }
+        } else if (g.res) {
+          // (rows that no tensor map takes: 2 byte loads, 32 of them on their way)
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 16) {
+            __half v[16][2];
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const bool in = row0 + r0 + r < g.M && c + lane + 32 * h < nc;
+                v[r][h] = in ? g.res[(row0 + r0 + r) * g.rs + n0 + c + lane + 32 * h] : __half();
+              }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) *staged(r0 + r, lane + 32 * h) = v[r][h];
+          }
+          __syncwarp();
+        }
+      };
+      if (live) prepare(0);  // (under the tile's products)
+      ok = mbar_wait(base + HDR_TFULL + 8 * my_buf, my_ph, abort_flag, g.status, 13);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (uint32_t)(my_buf * g.BN) + ((uint32_t)(q * 32) << 16);
+      for (int c = 0; live && c < nc; c += 64) {
+        if (c > 0) prepare(c);
         if (g.res_tma) {
           ok = mbar_wait(rbar, rph, abort_flag, g.status, 15);
           rph ^= 1;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-        } else if (g.res) {
-          for (int r = 0; r < 32 && row0 + r < g.M; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int j = lane + 32 * h;
-              if (c + j < nc)
-                *reinterpret_cast<__half *>(stg_p + r * 128 + ((((j >> 3) ^ (r & 7)) << 4) | ((j & 7) << 1))) =
-                    g.res[(row0 + r) * g.rs + n0 + c + j];
-            }
-          __syncwarp();
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -483,14 +564,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
           }
         } else {
           __syncwarp();
-          for (int r = 0; r < 32 && row0 + r < g.M; ++r)
+#pragma unroll 8
+          for (int r = 0; r < 32; ++r)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int j = lane + 32 * h;
-              if (c + j < nc)
-                g.out[(row0 + r) * g.os + n0 + c + j] =
-                    *reinterpret_cast<const __half *>(stg_p + r * 128 + ((((j >> 3) ^ (r & 7)) << 4) | ((j & 7) << 1)));
-            }
+            for (int h = 0; h < 2; ++h)
+              if (row0 + r < g.M && c + lane + 32 * h < nc)
+                g.out[(row0 + r) * g.os + n0 + c + lane + 32 * h] = *staged(r, lane + 32 * h);
           fence_proxy_async();  // (the next residual box comes through the copy engine)
         }
         __syncwarp();
@@ -499,7 +578,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        const uint32_t te = base + HDR_TEMPTY + 8 * buf;
+        const uint32_t te = base + HDR_TEMPTY + 8 * my_buf;
         if (CG == 2) mbar_arrive_cluster(map_rank(te, 0));
         else mbar_arrive(te);
       }
@@ -517,24 +596,42 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) linear_tile(const __grid_cons
 
 // ---- SPLIT ------------------------------------------------------------------
 // One tile of 128 output channels x BN rows per cluster; block r of the cluster takes the r-th part of c_in.  The
-// accumulator's lanes are output channels, its columns rows of x.  Partial sums go to the block's own shared memory (over
-// the operand stages, all read by then) as [row][128 channels]; each block then adds up its share of the items over the
-// cluster in rank order and writes them.
+// accumulator's lanes are output channels, its columns rows of x.  Rows are dealt out over the cluster for the epilogue:
+// every block sends each row's partial sums to the block that finishes it (distributed shared memory, [source][row][128
+// channels]), and that block adds them in rank order, so the bits do not depend on timing.  Sending instead of fetching
+// leaves one cluster barrier on the path and none at the end (the receiving block's own memory is all that is read).
 constexpr int SPLIT_THREADS = 256;
+constexpr int SPLIT_FIXED = HEADER + 1024;  // header, x scales of the block's rows
 
 template <bool F8>
 __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_constant__ LinArgs g) {
   extern __shared__ uint8_t dyn[];
   const uint32_t base = aligned_base(dyn);
   uint8_t *hdr = dyn + (base - smem_u32(dyn));
+  float *s_xs = reinterpret_cast<float *>(hdr + HEADER);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(hdr + HDR_ABORT);
   const int S = g.split, rank = (int)blockIdx.x % S, ft = (int)blockIdx.x / S;
   const int n0 = ft * 128, m0 = (int)blockIdx.y * g.BN;
   const int kb0 = (int)((long long)g.kb * rank / S), kb1 = (int)((long long)g.kb * (rank + 1) / S);
-  const uint32_t stage_bytes = 16384u + (uint32_t)g.BN * 128u, stage0 = base + HEADER;
+  const uint32_t stage_bytes = 16384u + (uint32_t)g.BN * 128u, stage0 = base + SPLIT_FIXED;
+  const uint32_t recv = stage0 + (g.overlay ? 0u : stage_bytes * (uint32_t)g.stages);
   const uint32_t cols = g.BN <= 32 ? 32u : g.BN <= 64 ? 64u : g.BN <= 128 ? 128u : 256u;
+  const int rows = min(g.BN, g.M - m0), per = (rows + S - 1) / S;  // this tile's rows; rows a block finishes
+  const int mine = max(0, min(per, rows - rank * per));
 
+  // The steps are walked from a start that differs from tile to tile: blocks that stream rows of the same pitch in step
+  // would all ask for the same columns, the same few memory channels, at once.
+  const int nkb = kb1 - kb0, rot = (ft * 5) % nkb;
+  const auto step_of = [&](int i) { return kb0 + (i + rot < nkb ? i + rot : i + rot - nkb); };
+  const auto fetch = [&](int i, int s) {
+    const uint32_t full = base + HDR_FULL + 8 * s, a = stage0 + stage_bytes * (uint32_t)s;
+    const int x = step_of(i) * (F8 ? 128 : 64);
+    mbar_expect_tx(full, stage_bytes);
+    tma_load_2d<1>(a, &g.tm_w, x, n0, full);
+    tma_load_2d<1>(a + 16384u, &g.tm_x, x, m0, full);
+  };
+  const int early = min(2, nkb);
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     *reinterpret_cast<volatile unsigned long long *>(abort_flag + 1) = g.wait_limit;
@@ -544,23 +641,33 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
     }
     mbar_init(base + HDR_TFULL, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // the first copies need nothing but the barriers: they are on their way while the rest is set up
+    for (int i = 0; i < early; ++i) fetch(i, i);
   }
   if (warp == 2) tmem_alloc<1>(base + HDR_TMEM, cols);
+  if (warp == 3)
+    for (int i = lane; i < mine; i += 32) s_xs[i] = g.x_scale ? __ldg(g.x_scale + m0 + rank * per + i) : 1.0f;
+  // the four channels this thread will finish, in every row it finishes
+  const int f = lane * 4, n = n0 + f;
+  float bias[4], wsc[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    bias[e] = g.bias && n + e < g.N ? __half2float(__ldg(g.bias + n + e)) : 0.0f;
+    wsc[e] = g.w_scale && n + e < g.N ? __ldg(g.w_scale + n + e) : 1.0f;
+  }
   tc_fence_before();
   __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for before the first remote store)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(hdr + HDR_TMEM);
 
   if (warp == 0) {
     if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 1;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      int s = early % g.stages;
+      uint32_t ph = early < g.stages ? 1 : 0;
+      for (int i = early; i < nkb; ++i) {
         if (!mbar_wait(base + HDR_EMPTY + 8 * s, ph, abort_flag, g.status, 12)) break;
-        const uint32_t full = base + HDR_FULL + 8 * s, a = stage0 + stage_bytes * (uint32_t)s;
-        mbar_expect_tx(full, stage_bytes);
-        tma_load_2d<1>(a, &g.tm_w, kb * (F8 ? 128 : 64), n0, full);
-        tma_load_2d<1>(a + 16384u, &g.tm_x, kb * (F8 ? 128 : 64), m0, full);
+        fetch(i, s);
         if (++s == g.stages) {
           s = 0;
           ph ^= 1;
@@ -573,13 +680,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int i = 0; i < nkb; ++i) {
         ok = mbar_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
         if (!ok) break;
         tc_fence_after();
         const uint64_t a = operand_desc(stage0 + stage_bytes * (uint32_t)s), b = a + (16384u >> 4);
-        const int ks = k_steps<F8>(g, kb);
-        for (int k = 0; k < ks; ++k) mma_step<1, F8>(tmem, a + 2 * k, b + 2 * k, idesc, kb > kb0 || k > 0);
+        const int ks = k_steps<F8>(g, step_of(i));
+        for (int k = 0; k < ks; ++k) mma_step<1, F8>(tmem, a + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
         mma_commit<1>(base + HDR_EMPTY + 8 * s);
         if (++s == g.stages) {
           s = 0;
@@ -592,58 +699,66 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
   __syncwarp();
   bool ok = mbar_wait(base + HDR_TFULL, 0, abort_flag, g.status, 13);
   ok = __all_sync(0xffffffffu, ok);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (g.overlay) cluster_sync();  // the received rows lie over the stages: every block is done with its own
   if (ok) {
     tc_fence_after();
     const int q = warp & 3;
-    for (int c = (warp >> 2) * 16; c < g.BN; c += 32) {
+    for (int c = (warp >> 2) * 16; c < rows; c += 32) {
       uint32_t raw[16];
       tc_ld16(tmem + (uint32_t)c + ((uint32_t)(q * 32) << 16), raw);
       tc_wait_ld();
-      const uint32_t dst = stage0 + (uint32_t)(c * 128 + q * 32 + lane) * 4u;
+      int to = c / per, r = c - to * per;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + (uint32_t)i * 512u), "r"(raw[i]) : "memory");
+      for (int i = 0; i < 16; ++i) {
+        if (c + i < rows) {
+          const uint32_t at = recv + (uint32_t)((rank * per + r) * 128 + q * 32 + lane) * 4u;
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_rank(at, (uint32_t)to)), "r"(raw[i]) : "memory");
+        }
+        if (++r == per) {
+          r = 0;
+          ++to;
+        }
+      }
     }
   }
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // (every block of the cluster comes here, aborted or not)
   tc_fence_after();
   abort_drain(abort_flag);
-  cluster_sync();  // (every block of the cluster comes here, aborted or not)
   if (warp == 2) tmem_free<1>(tmem, cols);
-  const int rows = min(g.BN, g.M - m0);
-  // 32 items of 4 channels per row: a warp writes 128 consecutive channels
-  for (int i = rank * SPLIT_THREADS + (int)threadIdx.x; i < rows * 32; i += S * SPLIT_THREADS) {
-    const int r = i >> 5, f = (i & 31) * 4, n = n0 + f;
+  const bool whole = n + 4 <= g.N && !((g.os | n0) & 3) && !((uintptr_t)g.out & 7);  // four channels by one store
+#pragma unroll 2
+  for (int r = warp; r < mine; r += SPLIT_THREADS / 32) {
     if (n >= g.N) continue;
-    const uint32_t at = stage0 + (uint32_t)(r * 128 + f) * 4u;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const long long m = m0 + rank * per + r;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, res[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) res[e] = g.res && n + e < g.N ? __half2float(g.res[m * g.rs + n + e]) : 0.0f;
     for (int b = 0; b < S; ++b) {
-      float4 p;
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
-                   : "r"(map_rank(at, (uint32_t)b)));
-      v[0] += p.x;
-      v[1] += p.y;
-      v[2] += p.z;
-      v[3] += p.w;
+      const uint4 p = lds128(recv + (uint32_t)((b * per + r) * 128 + f) * 4u);
+      v[0] += __uint_as_float(p.x);
+      v[1] += __uint_as_float(p.y);
+      v[2] += __uint_as_float(p.z);
+      v[3] += __uint_as_float(p.w);
     }
-    const long long m = m0 + r;
-    const float xs = g.x_scale ? __ldg(g.x_scale + m) : 1.0f;
+    const float xs = s_xs[r];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[e] = n + e < g.N ? fmaf(v[e] * xs, g.w_scale ? __ldg(g.w_scale + n + e) : 1.0f,
-                                g.bias ? __half2float(__ldg(g.bias + n + e)) : 0.0f)
-                         : 0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(v[e] * xs, wsc[e], bias[e]);
     activate(v, g.act, g.alpha);
+    if (g.res) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < g.N) {
-        const float r0 = g.res ? __half2float(g.res[m * g.rs + n + e]) : 0.0f;
-        g.out[m * g.os + n + e] = __float2half_rn(g.res ? v[e] + r0 : v[e]);
-      }
+      for (int e = 0; e < 4; ++e) v[e] += res[e];
+    }
+    __half *o = g.out + m * g.os + n;
+    if (whole) {
+      *reinterpret_cast<uint2 *>(o) = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < g.N) o[e] = __float2half_rn(v[e]);
+    }
   }
-  cluster_sync();  // no block leaves while another reads its partial sums
 }
 
 // ---- ROWS -------------------------------------------------------------------
@@ -676,14 +791,6 @@ template <bool F8>
 struct Piece {
   uint4 v[F8 ? 1 : 2];
 };
-template <bool F8>
-__device__ __forceinline__ void load_piece(Piece<F8> &p, const uint8_t *row, int chunk, int t, int kbytes, bool stream) {
-#pragma unroll
-  for (int i = 0; i < (F8 ? 1 : 2); ++i) {
-    const int at = chunk * (F8 ? 64 : 128) + i * 64 + t * 16;
-    p.v[i] = at < kbytes ? (stream ? ld_stream(row + at) : __ldg(reinterpret_cast<const uint4 *>(row + at))) : make_uint4(0, 0, 0, 0);
-  }
-}
 // The two registers (4 channels) that the piece gives to MMA step `s` of 4.
 template <bool F8>
 __device__ __forceinline__ void step_regs(const Piece<F8> &p, int s, uint32_t &r0, uint32_t &r1) {
@@ -699,13 +806,52 @@ __device__ __forceinline__ void step_regs(const Piece<F8> &p, int s, uint32_t &r
 }
 
 template <bool F8, int NT>
-__global__ void __launch_bounds__(ROWS_THREADS) linear_rows(const __grid_constant__ LinArgs g) {
-  constexpr int U = NT == 1 ? 4 : 2;  // chunks in flight
+struct RowsChunk {
+  Piece<F8> a, b, x[NT];
+};
+template <bool F8, int NT, bool TAIL>
+__device__ __forceinline__ void rows_load(RowsChunk<F8, NT> &r, const uint8_t *w0, const uint8_t *w1, const uint8_t *const (&xr)[NT],
+                                          const bool (&have)[NT], int chunk, int t, int kbytes) {
+#pragma unroll
+  for (int i = 0; i < (F8 ? 1 : 2); ++i) {
+    const int at = chunk * (F8 ? 64 : 128) + i * 64 + t * 16;
+    const bool in = !TAIL || at < kbytes;
+    r.a.v[i] = r.b.v[i] = make_uint4(0, 0, 0, 0);
+    if (in) {
+      r.a.v[i] = ld_stream(w0 + at);
+      r.b.v[i] = ld_stream(w1 + at);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      r.x[n].v[i] = make_uint4(0, 0, 0, 0);
+      if (in && have[n]) r.x[n].v[i] = __ldg(reinterpret_cast<const uint4 *>(xr[n] + at));
+    }
+  }
+}
+template <bool F8, int NT>
+__device__ __forceinline__ void rows_mma(const RowsChunk<F8, NT> &r, float (&acc)[NT][4]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    uint32_t a0, a1, a2, a3;
+    step_regs<F8>(r.a, s, a0, a2);
+    step_regs<F8>(r.b, s, a1, a3);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint32_t b0, b1;
+      step_regs<F8>(r.x[n], s, b0, b1);
+      mma_16816(acc[n], a0, a1, a2, a3, b0, b1);
+    }
+  }
+}
+
+template <bool F8, int NT>
+__global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows(const __grid_constant__ LinArgs g) {
+  constexpr int U = NT == 1 ? 4 : F8 ? 4 : 2;  // chunks in flight
   __shared__ float part[8][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
   const int f0 = (int)blockIdx.x * 16;
   const int kbytes = F8 ? g.K : 2 * g.K;
-  const int chunks = (g.K + 63) / 64;
+  const int chunks = (g.K + 63) / 64, whole = g.K / 64;
   const uint8_t *w0 = g.w + (long long)min(f0 + gr, g.N - 1) * g.ws, *w1 = g.w + (long long)min(f0 + gr + 8, g.N - 1) * g.ws;
   const uint8_t *xr[NT];
   bool have[NT];
@@ -715,30 +861,18 @@ __global__ void __launch_bounds__(ROWS_THREADS) linear_rows(const __grid_constan
     xr[n] = g.x + (have[n] ? (long long)(n * 8 + gr) * g.xs : 0);
   }
   float acc[NT][4] = {};
-  for (int c0 = warp; c0 < chunks; c0 += 8 * U) {
-    Piece<F8> a[U], b[U], x[U][NT];
+  int c = warp;
+  for (; c + 8 * (U - 1) < whole; c += 8 * U) {
+    RowsChunk<F8, NT> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = c0 + 8 * u;  // (beyond the last chunk: zeros)
-      load_piece<F8>(a[u], w0, c, t, kbytes, true);
-      load_piece<F8>(b[u], w1, c, t, kbytes, true);
+    for (int u = 0; u < U; ++u) rows_load<F8, NT, false>(r[u], w0, w1, xr, have, c + 8 * u, t, kbytes);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) load_piece<F8>(x[u][n], xr[n], c, t, have[n] ? kbytes : 0, false);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        uint32_t a0, a1, a2, a3;
-        step_regs<F8>(a[u], s, a0, a2);
-        step_regs<F8>(b[u], s, a1, a3);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint32_t b0, b1;
-          step_regs<F8>(x[u][n], s, b0, b1);
-          mma_16816(acc[n], a0, a1, a2, a3, b0, b1);
-        }
-      }
+    for (int u = 0; u < U; ++u) rows_mma<F8, NT>(r[u], acc);
+  }
+  for (; c < chunks; c += 8) {
+    RowsChunk<F8, NT> r;
+    rows_load<F8, NT, true>(r, w0, w1, xr, have, c, t, kbytes);
+    rows_mma<F8, NT>(r, acc);
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -911,18 +1045,29 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
     if (a.N > bn && bn % 64) bn = round_up(bn, 64);
   }
   const int cg = pair ? 2 : 1;
+  // The weights pass through L2 once per group of rows, so a group is as many rows as keep 36 MB of x (of 126 MB of L2)
+  // in flight, 4 to 32 tiles.  8192 x 4096 x 16384 binary16, 16 tiles against 8: 335 against 604 MB from memory, 942
+  // against 955 us under the power limit; 8192 x 8192 x 8192, where 16 tiles are 67 MB: 990 against 975 us.
+  const long long tile_bytes = 128ll * cg * a.K * r.es;
+  a.group = (int)(36000000ll / tile_bytes);
+  a.group = a.group < 4 ? 4 : a.group > 32 ? 32 : a.group;
   a.BN = bn;
   a.mt = (int)((a.M + 128ll * cg - 1) / (128 * cg));
   a.nt = (a.N + bn - 1) / bn;
-  const uint32_t stage = 16384u + (uint32_t)(bn / cg) * 128u;
-  const uint32_t fixed = 1024u + TILE_FIXED + 8u * STAGING;
+  a.bufs = bn <= 128 ? 4 : 2;
+  // two epilogue teams where a tile's products are soon done; one, and a stage more, where they take long
+  a.teams = a.kb >= 16 && !any ? 1 : 2;
+  const uint32_t wbytes = (uint32_t)(bn / cg) * 128u;
+  a.w_res = cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536;
+  const uint32_t stage = 16384u + (a.w_res ? 0u : wbytes);
+  const uint32_t fixed = 1024u + TILE_FIXED + 4u * (uint32_t)a.teams * STAGING + (a.w_res ? (uint32_t)a.kb * wbytes : 0u);
   a.stages = (int)((kSmemLimit - fixed) / stage);
   if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
   p->smem = fixed + stage * (uint32_t)a.stages;
   const long long tiles = (long long)a.mt * a.nt;
   const int clusters = (int)(tiles < sms / cg ? tiles : sms / cg);
   p->grid = dim3((unsigned)(clusters * cg));
-  p->block = dim3(TILE_THREADS);
+  p->block = dim3(any ? ANY_THREADS : TILE_THREADS);
   p->cluster = (uint32_t)cg;
   if (any) p->kernel = r.f8 ? (const void *)linear_tile<1, true, true> : (const void *)linear_tile<1, false, true>;
   else if (pair) p->kernel = r.f8 ? (const void *)linear_tile<2, true, false> : (const void *)linear_tile<2, false, false>;
@@ -934,20 +1079,32 @@ void plan_split(const Rec &r, int sms, dnxcu_linear_plan *p) {
   a.BN = a.M >= 256 ? 256 : round_up(a.M, 16);
   a.mt = (a.M + a.BN - 1) / a.BN;
   a.nt = (a.N + 127) / 128;
+  // the split with the fewest steps on the busiest SM, the smaller one of equals
   const long long tiles = (long long)a.mt * a.nt;
-  int s = 1;
-  while (s < 8 && s < a.kb && tiles * s < sms) ++s;
-  if (s > a.kb) s = a.kb;
-  a.split = s;
-  const uint32_t stage = 16384u + (uint32_t)a.BN * 128u, part = (uint32_t)a.BN * 512u;
-  int st = (int)((kSmemLimit / 2 - 2048u) / stage);  // two blocks per SM where that leaves enough stages
-  if (st < 3) st = (int)((kSmemLimit - 2048u) / stage);
-  a.stages = st > MAX_STAGES ? MAX_STAGES : st;
+  long long best = 0;
+  for (int s = 1; s <= 8 && s <= a.kb; ++s) {
+    const long long cost = (tiles * s + sms - 1) / sms * ((a.kb + s - 1) / s);
+    if (s == 1 || cost < best) {
+      best = cost;
+      a.split = s;
+    }
+  }
+  const uint32_t stage = 16384u + (uint32_t)a.BN * 128u, fixed = 1024u + SPLIT_FIXED;
+  const int most = a.BN < a.M ? a.BN : a.M, per = (most + a.split - 1) / a.split;
+  const uint32_t recv = (uint32_t)(a.split * per) * 512u;
+  // two blocks per SM where there are more blocks than SMs and shared memory leaves both some stages
+  uint32_t room = kSmemLimit - fixed;
+  if (tiles * a.split > sms && kSmemLimit / 2 - fixed - 1024u >= recv + 3 * stage) room = kSmemLimit / 2 - fixed - 1024u;
+  a.overlay = recv + 3 * stage > room;
+  int st = (int)((room - (a.overlay ? 0u : recv)) / stage);
+  const int steps = (a.kb + a.split - 1) / a.split;
+  st = st > MAX_STAGES ? MAX_STAGES : st;
+  a.stages = st > steps ? (steps > 2 ? steps : 2) : st;
   const uint32_t body = stage * (uint32_t)a.stages;
-  p->smem = 2048u + (body > part ? body : part);
-  p->grid = dim3((unsigned)(a.nt * s), (unsigned)a.mt);
+  p->smem = fixed + (a.overlay ? (body > recv ? body : recv) : body + recv);
+  p->grid = dim3((unsigned)(a.nt * a.split), (unsigned)a.mt);
   p->block = dim3(SPLIT_THREADS);
-  p->cluster = (uint32_t)s;
+  p->cluster = (uint32_t)a.split;
   p->kernel = r.f8 ? (const void *)linear_split<true> : (const void *)linear_split<false>;
 }
 
