@@ -200,8 +200,8 @@ __device__ __forceinline__ uint32_t aligned_base(const void *dyn) { return (smem
 // ---- TILE and ANY -----------------------------------------------------------
 // Warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7 and 8-11 are two epilogue teams that take
 // alternate tiles (or one team takes all); 2 or 4 accumulators rotate, so tiles are multiplied while the teams finish the
-// ones before.  ANY: warps 12-15 fetch with plain loads instead, each a whole stage, so four stages are on their way at
-// any time.  Where all of c_out is one column of tiles and the weights are small (a pointwise layer over pixels), they are
+// ones before.  ANY: seven warps (0, 2, 3, 12-15) fetch with plain loads instead, each a whole stage, so that as many
+// stages are on their way at any time.  Where all of c_out is one column of tiles and the weights are small (a pointwise layer over pixels), they are
 // fetched once per block and only rows of x stream.
 constexpr int TILE_THREADS = 384, ANY_THREADS = 512;
 constexpr int COLBUF = 512;              // per epilogue warp: bias and weight scale of 64 channels
@@ -220,25 +220,25 @@ __device__ __forceinline__ TilePos tile_pos(const LinArgs &g, int t) {
   return {m0 + r - n * gm, n};
 }
 
-// 16 bytes of an operand row at any alignment, zero beyond the row's end.  `begin` and `end` bound the whole operand: the
-// aligned 16 byte words around the piece are read where they lie inside it (between rows there are bytes of the same
-// buffer) and shifted together; at the operand's two ends single elements are read instead.
+// 16 bytes of an operand row at any alignment, zero beyond the row's end.  The aligned 16 byte words around the piece are
+// read (between rows there are bytes of the same buffer) and shifted together; where such a word would reach outside the
+// operand (`begin`, `end`: only at its two ends), single elements are read instead.
 struct PieceReq {
   uint4 a, b;
   const uint8_t *p;
-  int left;
+  int left;  // bytes of the row from the piece on
   bool slow;
 };
-__device__ __forceinline__ void request_piece(PieceReq &q, const uint8_t *row, int kbyte, int kbytes, const uint8_t *begin,
+__device__ __forceinline__ void request_piece(PieceReq &q, const uint8_t *p, int left, bool edge, const uint8_t *begin,
                                               const uint8_t *end) {
-  q.left = row ? kbytes - kbyte : 0;
-  q.p = row + kbyte;
+  q.left = left;
+  q.p = p;
   q.a = q.b = make_uint4(0, 0, 0, 0);
   q.slow = false;
-  if (q.left <= 0) return;
-  const int sh = (int)((uintptr_t)q.p & 15), need = sh + (q.left < 16 ? q.left : 16);
-  const uint8_t *w = q.p - sh;
-  q.slow = w < begin || w + (need > 16 ? 32 : 16) > end;
+  if (left <= 0) return;
+  const int sh = (int)((uintptr_t)p & 15), need = sh + min(left, 16);
+  const uint8_t *w = p - sh;
+  if (edge) q.slow = w < begin || w + (need > 16 ? 32 : 16) > end;
   if (q.slow) return;
   q.a = __ldg(reinterpret_cast<const uint4 *>(w));
   if (need > 16) q.b = __ldg(reinterpret_cast<const uint4 *>(w + 16));
@@ -266,35 +266,50 @@ __device__ __forceinline__ uint4 finish_piece(const PieceReq &q) {
   for (int i = 0; i < 5; ++i) w[i] = sh & 4 ? w[i + 1] : w[i];
   uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    o[i] = __funnelshift_r(w[i], w[i + 1], (sh & 3) * 8);
-    const int keep = q.left - i * 4;  // bytes of this word that lie inside the row
-    if (keep < 4) o[i] = keep <= 0 ? 0u : o[i] & (0xffffffffu >> (32 - 8 * keep));
+  for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(w[i], w[i + 1], (sh & 3) * 8);
+  if (q.left < 16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int keep = q.left - i * 4;  // bytes of this word that lie inside the row
+      if (keep < 4) o[i] = keep <= 0 ? 0u : o[i] & (0xffffffffu >> (32 - 8 * keep));
+    }
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
-// One warp fills `rows` rows (from row `row0` of an operand of `n` rows) of a swizzled tile with `pieces` pieces each.
-template <bool F8>
-__device__ __forceinline__ void fill_tile(uint32_t dst, const uint8_t *op, long long stride, long long row0, int n, int rows,
-                                          int pieces, int kb, int kbytes, int lane, int first, int step) {
-  const uint8_t *end = op + (long long)(n - 1) * stride + kbytes;
-  const int items = rows * pieces;
-  constexpr int B = 4;
+// One warp fills `rows` rows (from row `row0` of an operand of `n` rows) of a swizzled tile: the first 2^LP 16 byte pieces
+// of 128 byte step `kb` of each; of `step` warps that share the tile it is number `first`.
+template <bool F8, int LP>
+__device__ __forceinline__ void fill_pieces(uint32_t dst, const uint8_t *op, long long stride, long long row0, int n, int rows,
+                                            int kb, int kbytes, int lane, int first, int step) {
+  const uint8_t *end = op + (long long)(n - 1) * stride + kbytes, *at0 = op + row0 * stride + kb * 128;
+  const bool edge = row0 == 0 || row0 + rows >= n;
+  const int left_rows = (int)min((long long)rows, n - row0), items = rows << LP, left0 = kbytes - kb * 128;
+  constexpr int B = 8;
   for (int i0 = first * 32 + lane; i0 < items; i0 += 32 * step * B) {
     PieceReq q[B];
 #pragma unroll
     for (int u = 0; u < B; ++u) {
-      const int i = i0 + 32 * step * u, r = i / pieces, j = i - r * pieces;
-      request_piece(q[u], i < items && row0 + r < n ? op + (row0 + r) * stride : nullptr, kb * 128 + j * 16, kbytes, op, end);
+      const int i = i0 + 32 * step * u, r = i >> LP, j = i & ((1 << LP) - 1);
+      request_piece(q[u], at0 + r * stride + j * 16, r < left_rows ? left0 - j * 16 : 0, edge, op, end);
     }
 #pragma unroll
     for (int u = 0; u < B; ++u) {
-      const int i = i0 + 32 * step * u, r = i / pieces, j = i - r * pieces;
+      const int i = i0 + 32 * step * u, r = i >> LP, j = i & ((1 << LP) - 1);
       const uint4 v = finish_piece<F8>(q[u]);
       if (i < items) sts128(dst + (uint32_t)r * 128u + (uint32_t)((j ^ (r & 7)) << 4), v);
     }
   }
 }
+template <bool F8>
+__device__ __forceinline__ void fill_tile(uint32_t dst, const uint8_t *op, long long stride, long long row0, int n, int rows,
+                                          int ks, int kb, int kbytes, int lane, int first, int step) {
+  if (ks > 2) fill_pieces<F8, 3>(dst, op, stride, row0, n, rows, kb, kbytes, lane, first, step);
+  else if (ks == 2) fill_pieces<F8, 2>(dst, op, stride, row0, n, rows, kb, kbytes, lane, first, step);
+  else fill_pieces<F8, 1>(dst, op, stride, row0, n, rows, kb, kbytes, lane, first, step);
+}
+// ANY: the warps that fetch, numbered.
+constexpr int FETCHERS = 7;
+__device__ __forceinline__ int fetcher(int warp) { return warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : warp >= 12 ? warp - 9 : -1; }
 
 template <int CG, bool F8, bool ANY>
 __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
@@ -318,7 +333,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       mbar_init(base + HDR_EMPTY + 8 * i, 1);
     }
     for (int i = 0; i < 8; ++i) mbar_init(base + HDR_RES + 8 * i, 1);
-    mbar_init(base + HDR_WRES, ANY ? 4 : 1);
+    mbar_init(base + HDR_WRES, ANY ? FETCHERS : 1);
     for (int i = 0; i < MAX_BUFS; ++i) {
       mbar_init(base + HDR_TFULL + 8 * i, 1);
       mbar_init(base + HDR_TEMPTY + 8 * i, 4 * CG);
@@ -369,20 +384,23 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
         }
       }
     }
-  } else if (ANY && warp >= 12) {
+  } else if (ANY && fetcher(warp) >= 0) {
     // ---- operand tiles by plain loads, swizzled as the copy engine would ----
-    const int pw = warp - 12;
+    const int pw = fetcher(warp);
     const int kbytes = F8 ? g.K : 2 * g.K;
     if (g.w_res) {
       for (int kb = 0; kb < g.kb; ++kb)
-        fill_tile<F8>(wres0 + (uint32_t)kb * b_bytes, g.w, g.ws, 0, g.N, g.BN, 2 * k_steps<F8>(g, kb), kb, kbytes, lane, pw, 4);
+        fill_tile<F8>(wres0 + (uint32_t)kb * b_bytes, g.w, g.ws, 0, g.N, g.BN, k_steps<F8>(g, kb), kb, kbytes, lane, pw, FETCHERS);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(base + HDR_WRES);
     }
+    // At most as many warps take turns as there are stages: a warp that takes block j has then waited for block
+    // j - 2 * stages to be consumed, so the stage's barrier is at most one phase behind and its parity says enough.
+    const int turns = min(FETCHERS, g.stages);
     int s = 0, turn = 0;
     uint32_t ph = 1;
-    bool ok = true;
+    bool ok = pw < turns;
     for (int t = first; ok && t < ntiles; t += step) {
       const TilePos p = tile_pos(g, t);
       for (int kb = 0; kb < g.kb; ++kb) {
@@ -391,14 +409,14 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
           ok = __all_sync(0xffffffffu, ok);  // (the warp leaves the loop as one)
           if (!ok) break;
           const uint32_t a = stage0 + stage_bytes * (uint32_t)s;
-          const int pieces = 2 * k_steps<F8>(g, kb);  // 16 byte pieces of a row that the MMAs will read
-          fill_tile<F8>(a, g.x, g.xs, (long long)p.m * 128, g.M, 128, pieces, kb, kbytes, lane, 0, 1);
-          if (!g.w_res) fill_tile<F8>(a + 16384u, g.w, g.ws, (long long)p.n * g.BN, g.N, g.BN, pieces, kb, kbytes, lane, 0, 1);
+          const int ks = k_steps<F8>(g, kb);
+          fill_tile<F8>(a, g.x, g.xs, (long long)p.m * 128, g.M, 128, ks, kb, kbytes, lane, 0, 1);
+          if (!g.w_res) fill_tile<F8>(a + 16384u, g.w, g.ws, (long long)p.n * g.BN, g.N, g.BN, ks, kb, kbytes, lane, 0, 1);
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(base + HDR_FULL + 8 * s);
         }
-        turn = (turn + 1) & 3;
+        turn = turn + 1 == turns ? 0 : turn + 1;
         if (++s == g.stages) {
           s = 0;
           ph ^= 1;
@@ -474,6 +492,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       // What 64 channels need besides the sums: bias, scales and the residual, which goes into the staging tile.
       const auto prepare = [&](int c) {
         if (lane == 0) bulk_group_wait_read();  // the staging tile's last store has read it
+        if (g.nt > 1 || g.BN > 64 || it < 2)  // (else they are there from the team's first tile)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int j = lane + 32 * h, n = n0 + c + j;
@@ -804,86 +823,120 @@ __device__ __forceinline__ void step_regs(const Piece<F8> &p, int s, uint32_t &r
     r1 = s & 1 ? v.w : v.y;
   }
 }
-
-template <bool F8, int NT>
+// MT groups of 16 output channels, NT groups of 8 rows of x; w[i] and x[i] are the rows of the lane's group in them.
+template <bool F8, int NT, int MT>
 struct RowsChunk {
-  Piece<F8> a, b, x[NT];
+  Piece<F8> w[2 * MT], x[NT];
 };
-template <bool F8, int NT, bool TAIL>
-__device__ __forceinline__ void rows_load(RowsChunk<F8, NT> &r, const uint8_t *w0, const uint8_t *w1, const uint8_t *const (&xr)[NT],
-                                          const bool (&have)[NT], int chunk, int t, int kbytes) {
+template <bool F8, int NT, int MT>
+struct RowsPtr {
+  const uint8_t *w[2 * MT], *x[NT];
+  bool have[NT];
+};
+// TAIL: the row may end inside the chunk, at a 16 byte boundary.
+template <bool F8, int NT, int MT, bool TAIL>
+__device__ __forceinline__ void rows_load(RowsChunk<F8, NT, MT> &r, const RowsPtr<F8, NT, MT> &p, int chunk, int t, int kbytes) {
 #pragma unroll
   for (int i = 0; i < (F8 ? 1 : 2); ++i) {
     const int at = chunk * (F8 ? 64 : 128) + i * 64 + t * 16;
     const bool in = !TAIL || at < kbytes;
-    r.a.v[i] = r.b.v[i] = make_uint4(0, 0, 0, 0);
-    if (in) {
-      r.a.v[i] = ld_stream(w0 + at);
-      r.b.v[i] = ld_stream(w1 + at);
+#pragma unroll
+    for (int m = 0; m < 2 * MT; ++m) {
+      r.w[m].v[i] = make_uint4(0, 0, 0, 0);
+      if (in) r.w[m].v[i] = ld_stream(p.w[m] + at);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       r.x[n].v[i] = make_uint4(0, 0, 0, 0);
-      if (in && have[n]) r.x[n].v[i] = __ldg(reinterpret_cast<const uint4 *>(xr[n] + at));
+      if (in && p.have[n]) r.x[n].v[i] = __ldg(reinterpret_cast<const uint4 *>(p.x[n] + at));
     }
   }
 }
-template <bool F8, int NT>
-__device__ __forceinline__ void rows_mma(const RowsChunk<F8, NT> &r, float (&acc)[NT][4]) {
+template <bool F8, int NT, int MT>
+__device__ __forceinline__ void rows_mma(const RowsChunk<F8, NT, MT> &r, float (&acc)[MT][NT][4]) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    uint32_t a0, a1, a2, a3;
-    step_regs<F8>(r.a, s, a0, a2);
-    step_regs<F8>(r.b, s, a1, a3);
+  for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      uint32_t b0, b1;
-      step_regs<F8>(r.x[n], s, b0, b1);
-      mma_16816(acc[n], a0, a1, a2, a3, b0, b1);
+    for (int m = 0; m < MT; ++m) {
+      uint32_t a0, a1, a2, a3;
+      step_regs<F8>(r.w[2 * m], s, a0, a2);
+      step_regs<F8>(r.w[2 * m + 1], s, a1, a3);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint32_t b0, b1;
+        step_regs<F8>(r.x[n], s, b0, b1);
+        mma_16816(acc[m][n], a0, a1, a2, a3, b0, b1);
+      }
     }
-  }
 }
 
-template <bool F8, int NT>
+// U chunks of 64 channels are on their way per warp at any time.
+template <bool F8, int NT, int MT, int U, bool ANY>
 __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows(const __grid_constant__ LinArgs g) {
-  constexpr int U = NT == 1 ? 4 : F8 ? 4 : 2;  // chunks in flight
-  __shared__ float part[8][16][8 * NT + 1];
+  __shared__ float part[8][16 * MT][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
-  const int f0 = (int)blockIdx.x * 16;
+  const int f0 = (int)blockIdx.x * 16 * MT;
   const int kbytes = F8 ? g.K : 2 * g.K;
   const int chunks = (g.K + 63) / 64, whole = g.K / 64;
-  const uint8_t *w0 = g.w + (long long)min(f0 + gr, g.N - 1) * g.ws, *w1 = g.w + (long long)min(f0 + gr + 8, g.N - 1) * g.ws;
-  const uint8_t *xr[NT];
-  bool have[NT];
+  RowsPtr<F8, NT, MT> p;
+#pragma unroll
+  for (int m = 0; m < 2 * MT; ++m) p.w[m] = g.w + (long long)min(f0 + 8 * m + gr, g.N - 1) * g.ws;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    have[n] = n * 8 + gr < g.M;
-    xr[n] = g.x + (have[n] ? (long long)(n * 8 + gr) * g.xs : 0);
+    p.have[n] = n * 8 + gr < g.M;
+    p.x[n] = g.x + (p.have[n] ? (long long)(n * 8 + gr) * g.xs : 0);
   }
-  float acc[NT][4] = {};
+  float acc[MT][NT][4] = {};
   int c = warp;
-  for (; c + 8 * (U - 1) < whole; c += 8 * U) {
-    RowsChunk<F8, NT> r[U];
+  if (!ANY) {
+    for (; c + 8 * (U - 1) < whole; c += 8 * U) {
+      RowsChunk<F8, NT, MT> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) rows_load<F8, NT, false>(r[u], w0, w1, xr, have, c + 8 * u, t, kbytes);
+      for (int u = 0; u < U; ++u) rows_load<F8, NT, MT, false>(r[u], p, c + 8 * u, t, kbytes);
 #pragma unroll
-    for (int u = 0; u < U; ++u) rows_mma<F8, NT>(r[u], acc);
-  }
-  for (; c < chunks; c += 8) {
-    RowsChunk<F8, NT> r;
-    rows_load<F8, NT, true>(r, w0, w1, xr, have, c, t, kbytes);
-    rows_mma<F8, NT>(r, acc);
+      for (int u = 0; u < U; ++u) rows_mma<F8, NT, MT>(r[u], acc);
+    }
+    for (; c < chunks; c += 8) {
+      RowsChunk<F8, NT, MT> r;
+      rows_load<F8, NT, MT, true>(r, p, c, t, kbytes);
+      rows_mma<F8, NT, MT>(r, acc);
+    }
+  } else {
+    const uint8_t *wend = g.w + (long long)(g.N - 1) * g.ws + kbytes, *xend = g.x + (long long)(g.M - 1) * g.xs + kbytes;
+    for (; c < chunks; c += 8) {
+      constexpr int H = F8 ? 1 : 2;
+      PieceReq qw[2 * MT][H], qx[NT][H];
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const int at = c * (F8 ? 64 : 128) + i * 64 + t * 16;
+#pragma unroll
+        for (int m = 0; m < 2 * MT; ++m) request_piece(qw[m][i], p.w[m] + at, kbytes - at, true, g.w, wend);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) request_piece(qx[n][i], p.x[n] + at, p.have[n] ? kbytes - at : 0, true, g.x, xend);
+      }
+      RowsChunk<F8, NT, MT> r;
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+#pragma unroll
+        for (int m = 0; m < 2 * MT; ++m) r.w[m].v[i] = finish_piece<F8>(qw[m][i]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) r.x[n].v[i] = finish_piece<F8>(qx[n][i]);
+      }
+      rows_mma<F8, NT, MT>(r, acc);
+    }
   }
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    part[warp][gr][n * 8 + 2 * t] = acc[n][0];
-    part[warp][gr][n * 8 + 2 * t + 1] = acc[n][1];
-    part[warp][gr + 8][n * 8 + 2 * t] = acc[n][2];
-    part[warp][gr + 8][n * 8 + 2 * t + 1] = acc[n][3];
-  }
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      part[warp][16 * m + gr][n * 8 + 2 * t] = acc[m][n][0];
+      part[warp][16 * m + gr][n * 8 + 2 * t + 1] = acc[m][n][1];
+      part[warp][16 * m + gr + 8][n * 8 + 2 * t] = acc[m][n][2];
+      part[warp][16 * m + gr + 8][n * 8 + 2 * t + 1] = acc[m][n][3];
+    }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 8 * NT; i += ROWS_THREADS) {
-    const int f = i & 15, m = i >> 4, n = f0 + f;
+  for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += ROWS_THREADS) {
+    const int f = i % (16 * MT), m = i / (16 * MT), n = f0 + f;
     if (m >= g.M || n >= g.N) continue;
     float v[1] = {0.0f};
 #pragma unroll
@@ -893,6 +946,44 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows(const __grid_cons
     activate(v, g.act, g.alpha);
     if (g.res) v[0] += __half2float(g.res[m * g.rs + n]);
     g.out[m * g.os + n] = __float2half_rn(v[0]);
+  }
+}
+
+// ---- operands that no copy engine takes, laid out anew -----------------------
+// Rows of any alignment to rows on 16 byte boundaries (what lies behind a row's end in its last piece is zero).  x and the
+// weights in one launch: pieces [0, first) are the first operand's.
+struct RelayArgs {
+  const uint8_t *src[2];
+  uint8_t *dst[2];
+  long long stride[2], pitch[2], pieces[2];  // bytes per source row, per laid out row; 16 byte pieces in all
+  int rows[2], kbytes, per_row;              // pieces per row
+};
+template <bool F8>
+__global__ void __launch_bounds__(256) linear_relay(const RelayArgs g) {
+  constexpr int B = 4;
+  const long long n = g.pieces[0] + g.pieces[1];
+  for (long long i0 = (long long)blockIdx.x * 256 * B + threadIdx.x; i0 < n; i0 += (long long)gridDim.x * 256 * B) {
+    PieceReq q[B];
+    uint8_t *to[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      long long i = i0 + 256 * u;
+      const bool in = i < n;
+      const int o = in && i >= g.pieces[0];
+      if (o) i -= g.pieces[0];
+      // (a 64 bit division only where the pieces of an operand do not fit in 32)
+      const uint32_t row = !in ? 0u : i >> 32 ? (uint32_t)((unsigned long long)i / (unsigned)g.per_row) : (uint32_t)i / (unsigned)g.per_row;
+      const int at = (int)(i - (long long)row * g.per_row) * 16;
+      const uint8_t *src = g.src[o];
+      to[u] = in ? g.dst[o] + row * g.pitch[o] + at : nullptr;
+      request_piece(q[u], src + row * g.stride[o] + at, in ? g.kbytes - at : 0, true, src,
+                    src + (g.rows[o] - 1) * g.stride[o] + g.kbytes);
+    }
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const uint4 v = finish_piece<F8>(q[u]);
+      if (to[u]) *reinterpret_cast<uint4 *>(to[u]) = v;
+    }
   }
 }
 
@@ -986,7 +1077,7 @@ int pick(const Rec &r) {
     default: break;
   }
   if (!fits_tc(r)) return DNXCU_LINEAR_ANY;
-  if (r.d.rows <= 8 && fits_rows(r)) return DNXCU_LINEAR_ROWS;
+  if (fits_rows(r)) return DNXCU_LINEAR_ROWS;
   return r.d.rows <= 256 ? DNXCU_LINEAR_SPLIT : DNXCU_LINEAR_TILE;
 }
 
@@ -997,10 +1088,14 @@ using namespace dnxcu;
 
 struct dnxcu_linear_plan {
   LinArgs a;
+  RelayArgs relay;            // operands laid out anew in front of the kernel (scratch: where)
+  void *scratch = nullptr;
+  unsigned relay_grid = 0;
   const void *kernel = nullptr;
   dim3 grid, block;
   uint32_t smem = 0, cluster = 1;
   int device = 0, variant = 0;
+  bool f8 = false;
 };
 
 namespace dnxcu {
@@ -1108,20 +1203,65 @@ void plan_split(const Rec &r, int sms, dnxcu_linear_plan *p) {
   p->kernel = r.f8 ? (const void *)linear_split<true> : (const void *)linear_split<false>;
 }
 
-int make_plan(const Rec &r, dnxcu_linear_plan *p) {
+// Kernel, geometry and tensor maps of a checked record whose operands start at `x` and `w`, their rows `a.xs` and `a.ws`
+// bytes apart (the caller's, or the plan's aligned copies), for variant `v`.
+int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxcu_linear_plan *p) {
+  const dnxcu_linear &d = r.d;
+  LinArgs &a = p->a;
+  a.x = (const uint8_t *)x;
+  a.w = (const uint8_t *)w;
+  if (v == DNXCU_LINEAR_ROWS || (v == DNXCU_LINEAR_ANY && a.M <= 16)) {
+    p->block = dim3(ROWS_THREADS);
+    const bool two = a.M > 8;
+    int mt = 1;
+    if (v == DNXCU_LINEAR_ANY) {
+      if (r.f8) p->kernel = two ? (const void *)linear_rows<true, 2, 1, 1, true> : (const void *)linear_rows<true, 1, 1, 1, true>;
+      else p->kernel = two ? (const void *)linear_rows<false, 2, 1, 1, true> : (const void *)linear_rows<false, 1, 1, 1, true>;
+    } else if (r.f8 && (a.N + 15) / 16 > 3 * sms) {
+      // 8 bit weights and many channels: 32 per block, so that x is fetched half as often and blocks last longer
+      mt = 2;
+      p->kernel = two ? (const void *)linear_rows<true, 2, 2, 4, false> : (const void *)linear_rows<true, 1, 2, 4, false>;
+    } else if (r.f8) {
+      p->kernel = two ? (const void *)linear_rows<true, 2, 1, 4, false> : (const void *)linear_rows<true, 1, 1, 4, false>;
+    } else {
+      p->kernel = two ? (const void *)linear_rows<false, 2, 1, 2, false> : (const void *)linear_rows<false, 1, 1, 4, false>;
+    }
+    p->grid = dim3((unsigned)((a.N + 16 * mt - 1) / (16 * mt)));
+    return DNXCU_OK;
+  }
+  int st = init_device(p->device);
+  if (st) return st;
+  if (v == DNXCU_LINEAR_SPLIT) {
+    plan_split(r, sms, p);
+    st = matrix_map(&a.tm_w, w, r.f8, a.N, a.K, a.ws, 128);
+    return st ? st : matrix_map(&a.tm_x, x, r.f8, a.M, a.K, a.xs, a.BN);
+  }
+  plan_tile(r, sms, v == DNXCU_LINEAR_ANY, p);
+  if (v == DNXCU_LINEAR_TILE) {
+    st = matrix_map(&a.tm_x, x, r.f8, a.M, a.K, a.xs, 128);
+    if (!st) st = matrix_map(&a.tm_w, w, r.f8, a.N, a.K, a.ws, a.BN / (int)p->cluster);
+    if (st) return st;
+  }
+  a.out_tma = mappable(d.out, a.os * 2);
+  a.res_tma = d.residual && mappable(d.residual, a.rs * 2);
+  if (a.out_tma && (st = matrix_map(&a.tm_out, d.out, false, a.M, a.N, a.os * 2, 32))) return st;
+  if (a.res_tma && (st = matrix_map(&a.tm_res, d.residual, false, a.M, a.N, a.rs * 2, 32))) return st;
+  return DNXCU_OK;
+}
+
+// `keep`: the plan outlives this call and may hold scratch memory.
+int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
   const dnxcu_linear &d = r.d;
   const int v = pick(r);
   if (v < 0) return v;
-  p->variant = v;
   DNXCU_CUDA(cudaGetDevice(&p->device));
   for (const void *q : {d.x, d.weights, (const void *)d.x_scale, (const void *)d.w_scale, d.bias, d.residual, (const void *)d.out,
                         (const void *)d.device_status})
     if (!on_current_device(q)) return DNXCU_E_BAD_ARG;
   const int sms = sm_count(p->device);
+  p->f8 = r.f8;
   LinArgs &a = p->a;
   memset(&a, 0, sizeof(a));
-  a.x = (const uint8_t *)d.x;
-  a.w = (const uint8_t *)d.weights;
   a.x_scale = d.x_scale;
   a.w_scale = d.w_scale;
   a.bias = (const __half *)d.bias;
@@ -1136,38 +1276,51 @@ int make_plan(const Rec &r, dnxcu_linear_plan *p) {
   a.K = d.c_in;
   a.act = d.activation;
   a.alpha = d.leaky_alpha;
-  a.kb = (d.c_in * r.es + 127) / 128;
+  a.kb = (int)(((long long)d.c_in * r.es + 127) / 128);
   a.status = d.device_status;
   a.wait_limit = wait_limit_cycles();
   if (a.wait_limit < 2000000ull) a.wait_limit |= 1ull << 63;  // below about a millisecond: strict (see mbar_wait)
-  if (v == DNXCU_LINEAR_ROWS) {
-    p->grid = dim3((unsigned)((a.N + 15) / 16));
-    p->block = dim3(ROWS_THREADS);
-    if (r.f8) p->kernel = a.M <= 8 ? (const void *)linear_rows<true, 1> : (const void *)linear_rows<true, 2>;
-    else p->kernel = a.M <= 8 ? (const void *)linear_rows<false, 1> : (const void *)linear_rows<false, 2>;
-    return DNXCU_OK;
+  // Unaligned operands of a kept plan: laid out anew in scratch memory by one kernel, then the aligned variants.
+  if (v == DNXCU_LINEAR_ANY && d.variant == DNXCU_LINEAR_AUTO && keep && a.M > 16) {
+    RelayArgs &y = p->relay;
+    memset(&y, 0, sizeof(y));
+    const bool rx = !mappable(d.x, a.xs), rw = !mappable(d.weights, a.ws);
+    const long long pitch = ((long long)a.K * r.es + 15) / 16 * 16;
+    y.kbytes = a.K * r.es;
+    y.per_row = (int)(pitch / 16);
+    y.src[0] = (const uint8_t *)d.x;
+    y.src[1] = (const uint8_t *)d.weights;
+    y.stride[0] = a.xs;
+    y.stride[1] = a.ws;
+    y.rows[0] = a.M;
+    y.rows[1] = a.N;
+    y.pitch[0] = y.pitch[1] = pitch;
+    const size_t xb = rx ? (size_t)a.M * (size_t)pitch : 0, wb = rw ? (size_t)a.N * (size_t)pitch : 0;
+    y.pieces[0] = (long long)(xb / 16);
+    y.pieces[1] = (long long)(wb / 16);
+    if (cudaMalloc(&p->scratch, xb + wb) == cudaSuccess) {
+      y.dst[0] = (uint8_t *)p->scratch;
+      y.dst[1] = (uint8_t *)p->scratch + xb;
+      const long long blocks = (y.pieces[0] + y.pieces[1] + 1023) / 1024;
+      p->relay_grid = (unsigned)(blocks < 16ll * sms ? blocks : 16ll * sms);
+      if (rx) a.xs = pitch;
+      if (rw) a.ws = pitch;
+      p->variant = v;
+      return plan_kernel(r, a.M <= 256 ? DNXCU_LINEAR_SPLIT : DNXCU_LINEAR_TILE, rx ? y.dst[0] : d.x, rw ? y.dst[1] : d.weights, sms, p);
+    }
+    cudaGetLastError();  // (no room: the kernel that fetches by plain loads needs none)
+    p->scratch = nullptr;
   }
-  int st = init_device(p->device);
-  if (st) return st;
-  if (v == DNXCU_LINEAR_SPLIT) {
-    plan_split(r, sms, p);
-    st = matrix_map(&a.tm_w, d.weights, r.f8, a.N, a.K, a.ws, 128);
-    return st ? st : matrix_map(&a.tm_x, d.x, r.f8, a.M, a.K, a.xs, a.BN);
-  }
-  plan_tile(r, sms, v == DNXCU_LINEAR_ANY, p);
-  if (v == DNXCU_LINEAR_TILE) {
-    st = matrix_map(&a.tm_x, d.x, r.f8, a.M, a.K, a.xs, 128);
-    if (!st) st = matrix_map(&a.tm_w, d.weights, r.f8, a.N, a.K, a.ws, a.BN / (int)p->cluster);
-    if (st) return st;
-  }
-  a.out_tma = mappable(d.out, a.os * 2);
-  a.res_tma = d.residual && mappable(d.residual, a.rs * 2);
-  if (a.out_tma && (st = matrix_map(&a.tm_out, d.out, false, a.M, a.N, a.os * 2, 32))) return st;
-  if (a.res_tma && (st = matrix_map(&a.tm_res, d.residual, false, a.M, a.N, a.rs * 2, 32))) return st;
-  return DNXCU_OK;
+  p->variant = v;
+  return plan_kernel(r, v, d.x, d.weights, sms, p);
 }
 
 int launch(const dnxcu_linear_plan &p, cudaStream_t s) {
+  if (p.relay_grid) {
+    if (p.f8) linear_relay<true><<<p.relay_grid, 256, 0, s>>>(p.relay);
+    else linear_relay<false><<<p.relay_grid, 256, 0, s>>>(p.relay);
+    DNXCU_CUDA(cudaGetLastError());
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = p.grid;
   cfg.blockDim = p.block;
@@ -1208,7 +1361,7 @@ int dnxcu_linear_launch(const dnxcu_linear *d, void *stream) {
   int st = check(d, &r);
   if (st) return st;
   dnxcu_linear_plan p;
-  st = make_plan(r, &p);
+  st = make_plan(r, &p, false);
   return st ? st : launch(p, (cudaStream_t)stream);
 }
 
@@ -1219,9 +1372,9 @@ int dnxcu_linear_plan_create(const dnxcu_linear *d, dnxcu_linear_plan **out) {
   if (st) return st;
   dnxcu_linear_plan *p = new (std::nothrow) dnxcu_linear_plan();
   if (!p) return DNXCU_E_NO_MEMORY;
-  st = make_plan(r, p);
+  st = make_plan(r, p, true);
   if (st) {
-    delete p;
+    dnxcu_linear_plan_destroy(p);
     return st;
   }
   *out = p;
@@ -1236,6 +1389,16 @@ int dnxcu_linear_plan_launch(const dnxcu_linear_plan *p, void *stream) {
   return launch(*p, (cudaStream_t)stream);
 }
 
-void dnxcu_linear_plan_destroy(dnxcu_linear_plan *p) { delete p; }
+void dnxcu_linear_plan_destroy(dnxcu_linear_plan *p) {
+  if (!p) return;
+  if (p->scratch) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev != p->device) cudaSetDevice(p->device);
+    if (cudaFree(p->scratch) != cudaSuccess) cudaGetLastError();  // (waits for launches that still use it)
+    if (dev != p->device) cudaSetDevice(dev);
+  }
+  delete p;
+}
 
 }  // extern "C"

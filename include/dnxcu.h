@@ -327,7 +327,7 @@ typedef enum dnxcu_linear_variant {
   DNXCU_LINEAR_SPLIT = 2, /* few rows on the tensor cores: c_in split over the blocks of a cluster; x and weights on 16
                              byte boundaries with row strides that are multiples of 16 bytes */
   DNXCU_LINEAR_TILE = 3,  /* tiles of rows on the tensor cores; x and weights as for SPLIT */
-  DNXCU_LINEAR_ANY = 4    /* the tile kernel with operands fetched by plain loads: any alignment, any stride */
+  DNXCU_LINEAR_ANY = 4    /* ROWS and TILE with operands fetched by plain loads: any alignment, any stride */
 } dnxcu_linear_variant;
 
 typedef struct dnxcu_linear {
@@ -358,7 +358,11 @@ DNXCU_API int dnxcu_linear_pick(const dnxcu_linear *d);
 DNXCU_API int dnxcu_linear_launch(const dnxcu_linear *d, void *stream);
 /* The same planned once and launched many times, as dnxcu_plan_create does for a dispatch: checks, geometry and tensor
  * maps are worked out when the plan is made, on the device that is current then; launching it with another device
- * current is DNXCU_E_STATE.  A plan holds no device memory and may be launched on several streams. */
+ * current is DNXCU_E_STATE.  With AUTO and operands that break the alignment of SPLIT and TILE, a plan for more than 16
+ * rows holds scratch memory (allocated when it is made, so not during a stream capture) in which every launch first lays
+ * those operands out on 16 byte boundaries: many times faster than the kernel that a direct launch of them gets.  The
+ * caller owns the plan, keeps one per stream (or captured graph) that may launch concurrently, and destroys it after its
+ * last launch. */
 typedef struct dnxcu_linear_plan dnxcu_linear_plan;
 DNXCU_API int dnxcu_linear_plan_create(const dnxcu_linear *d, dnxcu_linear_plan **out);
 DNXCU_API int dnxcu_linear_plan_launch(const dnxcu_linear_plan *p, void *stream);

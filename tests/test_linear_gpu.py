@@ -247,6 +247,22 @@ def test_plan_streams_and_graph():
             assert torch.equal(o.cpu().double(), want)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "e4m3"])
+@pytest.mark.parametrize("m,k,n,strides,offsets", [(17, 9, 5, (0, 0), (0, 0)), (130, 65, 300, (0, 0), (0, 0)), (100, 1001, 129, (0, 0), (0, 0)),
+                                                   (1000, 27, 24, (0, 0), (0, 0)), (300, 64, 96, (65, 64), (0, 0)),
+                                                   (300, 64, 96, (64, 67), (0, 0)), (257, 96, 64, (96, 96), (3, 0)),
+                                                   (600, 513, 2000, (520, 515), (1, 5)), (1, 77, 40, (0, 0), (1, 1)),
+                                                   (9, 333, 20, (0, 0), (0, 3)), (4000, 1, 1, (0, 0), (0, 0))])
+def test_plan_of_unaligned_operands(m, k, n, strides, offsets, dtype):
+    """What a kept plan does with rows off 16 byte boundaries (scratch), and a direct call without any: both right."""
+    x, w, xs, ws = operands(dtype, m, k, n, 65)
+    b, r = normal(66, n), normal(67, m, n)
+    ref, tol = reference(x, w, xs, ws, b, r, "silu")
+    for planned in (True, False):
+        got = run(x, w, xs, ws, b, r, "silu", strides=strides + (0, 0), offsets=offsets + (0, 0), planned=planned)
+        assert_within(got, ref, tol, f"planned={planned}")
+
+
 def test_offsets_past_32_bits():
     """Rows of x and of the output that lie more than 2^32 elements from the first."""
     m, k, n, stride = 3, 64, 48, (1 << 31) + 8
