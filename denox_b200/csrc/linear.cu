@@ -135,6 +135,21 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uin
   else DNXCU_MMA("1", "f16");
 #undef DNXCU_MMA
 }
+// The `n` (1 to 4) steps of one stage, straight line code for each n: an MMA in a loop costs its thread about 200 cycles
+// of issue, one in straight line code about 60 (522240 rows, 32 to 32 channels: 22.0 us with a loop).
+template <int CG, bool F8, int N>
+__device__ __forceinline__ void mma_steps_n(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  mma_step<CG, F8>(d, a, b, idesc, accumulate);
+#pragma unroll
+  for (int k = 1; k < N; ++k) mma_step<CG, F8>(d, a + 2 * k, b + 2 * k, idesc, 1u);
+}
+template <int CG, bool F8>
+__device__ __forceinline__ void mma_steps(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, int n) {
+  if (n == 4) mma_steps_n<CG, F8, 4>(d, a, b, idesc, accumulate);
+  else if (n == 2) mma_steps_n<CG, F8, 2>(d, a, b, idesc, accumulate);
+  else if (n == 1) mma_steps_n<CG, F8, 1>(d, a, b, idesc, accumulate);
+  else mma_steps_n<CG, F8, 3>(d, a, b, idesc, accumulate);
+}
 // Arrives on `bar` (of both blocks of a pair) when the MMAs issued so far are done.
 template <int CG>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
@@ -190,7 +205,7 @@ __device__ __forceinline__ int k_steps(const LinArgs &g, int kb) {
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_BUFS = 4;  // accumulators in tensor memory
 constexpr int HDR_FULL = 0, HDR_EMPTY = 8 * MAX_STAGES, HDR_TFULL = 16 * MAX_STAGES, HDR_TEMPTY = HDR_TFULL + 8 * MAX_BUFS,
-              HDR_RES = HDR_TEMPTY + 8 * MAX_BUFS, HDR_WRES = HDR_RES + 64, HDR_TMEM = HDR_WRES + 8, HDR_ABORT = HDR_TMEM + 4;
+              HDR_RES = HDR_TEMPTY + 8 * MAX_BUFS, HDR_WRES = HDR_RES + 128, HDR_TMEM = HDR_WRES + 8, HDR_ABORT = HDR_TMEM + 4;
 static_assert((HDR_ABORT + 4) % 8 == 0 && HDR_ABORT + 12 <= 1024, "header layout");
 constexpr int HEADER = 1024;
 constexpr uint32_t kSmemLimit = 232448;
@@ -198,14 +213,15 @@ constexpr uint32_t kSmemLimit = 232448;
 __device__ __forceinline__ uint32_t aligned_base(const void *dyn) { return (smem_u32(dyn) + 1023u) & ~1023u; }
 
 // ---- TILE and ANY -----------------------------------------------------------
-// Warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7 and 8-11 are two epilogue teams that take
-// alternate tiles (or one team takes all); 2 or 4 accumulators rotate, so tiles are multiplied while the teams finish the
-// ones before.  ANY: seven warps (0, 2, 3, 12-15) fetch with plain loads instead, each a whole stage, so that as many
+// Warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7, 8-11, ... are one to four epilogue teams
+// that take turns; 2 or 4 accumulators rotate, so tiles are multiplied while the teams finish the ones before.  A team
+// needs about 2300 cycles for a tile of 32 channels whatever its products take (TMEM to registers to shared memory to the
+// copy engine, one after the other), so thin layers have four teams.  ANY: seven warps (0, 2, 3, 12-15) fetch with plain loads instead, each a whole stage, so that as many
 // stages are on their way at any time.  Where all of c_out is one column of tiles and the weights are small (a pointwise layer over pixels), they are
 // fetched once per block and only rows of x stream.
-constexpr int TILE_THREADS = 384, ANY_THREADS = 512;
+constexpr int PAIR_THREADS = 384, ONE_THREADS = 640, ANY_THREADS = 512;
 constexpr int COLBUF = 512;              // per epilogue warp: bias and weight scale of 64 channels
-constexpr int TILE_FIXED = HEADER + 8 * COLBUF;
+constexpr int TILE_FIXED = HEADER + 16 * COLBUF;
 constexpr int STAGING = 4096;            // per epilogue warp: 32 rows x 64 channels of binary16
 
 struct TilePos {
@@ -312,7 +328,7 @@ constexpr int FETCHERS = 7;
 __device__ __forceinline__ int fetcher(int warp) { return warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : warp >= 12 ? warp - 9 : -1; }
 
 template <int CG, bool F8, bool ANY>
-__global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
+__global__ void __launch_bounds__(ANY ? ANY_THREADS : CG == 2 ? PAIR_THREADS : ONE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
   extern __shared__ uint8_t dyn[];
   const uint32_t base = aligned_base(dyn);
   uint8_t *hdr = dyn + (base - smem_u32(dyn));
@@ -332,7 +348,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       mbar_init(base + HDR_FULL + 8 * i, 1);
       mbar_init(base + HDR_EMPTY + 8 * i, 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(base + HDR_RES + 8 * i, 1);
+    for (int i = 0; i < 16; ++i) mbar_init(base + HDR_RES + 8 * i, 1);
     mbar_init(base + HDR_WRES, ANY ? FETCHERS : 1);
     for (int i = 0; i < MAX_BUFS; ++i) {
       mbar_init(base + HDR_TFULL + 8 * i, 1);
@@ -427,6 +443,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
     // ---- MMA issue: one thread of the (first) block ----
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = mma_idesc(128 * CG, g.BN);
+      const int last = k_steps<F8>(g, g.kb - 1);
       int s = 0, buf = 0;
       uint32_t ph = 0, bph = 1;
       bool ok = !g.w_res || mbar_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
@@ -441,13 +458,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
           tc_fence_after();
           const uint32_t at = stage0 + stage_bytes * (uint32_t)s;
           const uint64_t a = operand_desc(at), b = operand_desc(g.w_res ? wres0 + (uint32_t)kb * b_bytes : at + 16384u);
-          const int ks = k_steps<F8>(g, kb);
-          if (ks == 4) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_step<CG, F8>(d, a + 2 * k, b + 2 * k, idesc, (kb | k) != 0);
-          } else {
-            for (int k = 0; k < ks; ++k) mma_step<CG, F8>(d, a + 2 * k, b + 2 * k, idesc, (kb | k) != 0);
-          }
+          mma_steps<CG, F8>(d, a, b, idesc, kb != 0, kb + 1 < g.kb ? 4 : last);
           mma_commit<CG>(base + HDR_EMPTY + 8 * s);
           if (++s == g.stages) {
             s = 0;
@@ -475,15 +486,18 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
     };
     uint32_t rph = 0, bph = 0;
     bool ok = true;
-    int it = 0, buf = 0;
-    for (int t = first; ok && t < ntiles; t += step, ++it) {
+    int turn = 0, buf = 0;
+    bool fresh = true;  // the team's first tile
+    for (int t = first; ok && t < ntiles; t += step) {
       const int my_buf = buf;
       const uint32_t my_ph = bph;
       if (++buf == g.bufs) {
         buf = 0;
         bph ^= 1;
       }
-      if (g.teams == 2 && (it & 1) != team) continue;
+      const bool ours = turn == team;
+      if (++turn == g.teams) turn = 0;
+      if (!ours) continue;
       const TilePos p = tile_pos(g, t);
       const int n0 = p.n * g.BN, nc = min(g.BN, g.N - n0);
       const long long row0 = (long long)p.m * (128 * CG) + (long long)rank * 128 + q * 32, row = row0 + lane;
@@ -492,7 +506,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       // What 64 channels need besides the sums: bias, scales and the residual, which goes into the staging tile.
       const auto prepare = [&](int c) {
         if (lane == 0) bulk_group_wait_read();  // the staging tile's last store has read it
-        if (g.nt > 1 || g.BN > 64 || it < 2)  // (else they are there from the team's first tile)
+        if (g.nt > 1 || g.BN > 64 || fresh)  // (else they are there from the team's first tile)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int j = lane + 32 * h, n = n0 + c + j;
@@ -526,6 +540,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
         }
       };
       if (live) prepare(0);  // (under the tile's products)
+      fresh = false;
       ok = mbar_wait(base + HDR_TFULL + 8 * my_buf, my_ph, abort_flag, g.status, 13);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -704,8 +719,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
         if (!ok) break;
         tc_fence_after();
         const uint64_t a = operand_desc(stage0 + stage_bytes * (uint32_t)s), b = a + (16384u >> 4);
-        const int ks = k_steps<F8>(g, step_of(i));
-        for (int k = 0; k < ks; ++k) mma_step<1, F8>(tmem, a + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
+        mma_steps<1, F8>(tmem, a, b, idesc, i > 0, k_steps<F8>(g, step_of(i)));
         mma_commit<1>(base + HDR_EMPTY + 8 * s);
         if (++s == g.stages) {
           s = 0;
@@ -746,36 +760,52 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
   tc_fence_after();
   abort_drain(abort_flag);
   if (warp == 2) tmem_free<1>(tmem, cols);
-  const bool whole = n + 4 <= g.N && !((g.os | n0) & 3) && !((uintptr_t)g.out & 7);  // four channels by one store
-#pragma unroll 2
-  for (int r = warp; r < mine; r += SPLIT_THREADS / 32) {
-    if (n >= g.N) continue;
-    const long long m = m0 + rank * per + r;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, res[4];
+  const bool whole = n + 4 <= g.N && !(g.os & 3) && !((uintptr_t)g.out & 7);  // four channels by one store
+  constexpr int R = 4, WARPS = SPLIT_THREADS / 32;  // rows a warp finishes at once
+  for (int r0 = warp; r0 < mine && n < g.N; r0 += R * WARPS) {
+    float v[4 * R], res[4 * R];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) res[e] = g.res && n + e < g.N ? __half2float(g.res[m * g.rs + n + e]) : 0.0f;
-    for (int b = 0; b < S; ++b) {
-      const uint4 p = lds128(recv + (uint32_t)((b * per + r) * 128 + f) * 4u);
-      v[0] += __uint_as_float(p.x);
-      v[1] += __uint_as_float(p.y);
-      v[2] += __uint_as_float(p.z);
-      v[3] += __uint_as_float(p.w);
+    for (int u = 0; u < R; ++u) {
+      const int r = r0 + u * WARPS;
+      const __half *rp = g.res + (long long)(m0 + rank * per + r) * g.rs + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) res[4 * u + e] = g.res && r < mine && n + e < g.N ? __half2float(rp[e]) : 0.0f;
     }
-    const float xs = s_xs[r];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fmaf(v[e] * xs, wsc[e], bias[e]);
+    for (int i = 0; i < 4 * R; ++i) v[i] = 0.0f;
+    for (int b = 0; b < S; ++b)
+#pragma unroll
+      for (int u = 0; u < R; ++u) {
+        const int r = min(r0 + u * WARPS, mine - 1);
+        const uint4 p = lds128(recv + (uint32_t)((b * per + r) * 128 + f) * 4u);
+        v[4 * u] += __uint_as_float(p.x);
+        v[4 * u + 1] += __uint_as_float(p.y);
+        v[4 * u + 2] += __uint_as_float(p.z);
+        v[4 * u + 3] += __uint_as_float(p.w);
+      }
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const float xs = s_xs[min(r0 + u * WARPS, mine - 1)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * u + e] = fmaf(v[4 * u + e] * xs, wsc[e], bias[e]);
+    }
     activate(v, g.act, g.alpha);
-    if (g.res) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += res[e];
-    }
-    __half *o = g.out + m * g.os + n;
-    if (whole) {
-      *reinterpret_cast<uint2 *>(o) = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
-    } else {
+    for (int u = 0; u < R; ++u) {
+      const int r = r0 + u * WARPS;
+      if (r >= mine) break;
+      if (g.res) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < g.N) o[e] = __float2half_rn(v[e]);
+        for (int e = 0; e < 4; ++e) v[4 * u + e] += res[4 * u + e];
+      }
+      __half *o = g.out + (long long)(m0 + rank * per + r) * g.os + n;
+      if (whole) {
+        *reinterpret_cast<uint2 *>(o) = make_uint2(pack_h2(v[4 * u], v[4 * u + 1]), pack_h2(v[4 * u + 2], v[4 * u + 3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < g.N) o[e] = __float2half_rn(v[4 * u + e]);
+      }
     }
   }
 }
@@ -1150,8 +1180,8 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   a.mt = (int)((a.M + 128ll * cg - 1) / (128 * cg));
   a.nt = (a.N + bn - 1) / bn;
   a.bufs = bn <= 128 ? 4 : 2;
-  // two epilogue teams where a tile's products are soon done; one, and a stage more, where they take long
-  a.teams = a.kb >= 16 && !any ? 1 : 2;
+  // more epilogue teams where a tile's products are soon done; one, and more stages, where they take long
+  a.teams = any || pair ? (a.kb >= 16 && pair ? 1 : 2) : a.kb >= 16 ? 1 : bn > 128 ? 2 : 4;
   const uint32_t wbytes = (uint32_t)(bn / cg) * 128u;
   a.w_res = cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536;
   const uint32_t stage = 16384u + (a.w_res ? 0u : wbytes);
@@ -1162,7 +1192,7 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   const long long tiles = (long long)a.mt * a.nt;
   const int clusters = (int)(tiles < sms / cg ? tiles : sms / cg);
   p->grid = dim3((unsigned)(clusters * cg));
-  p->block = dim3(any ? ANY_THREADS : TILE_THREADS);
+  p->block = dim3(any ? ANY_THREADS : pair ? PAIR_THREADS : ONE_THREADS);
   p->cluster = (uint32_t)cg;
   if (any) p->kernel = r.f8 ? (const void *)linear_tile<1, true, true> : (const void *)linear_tile<1, false, true>;
   else if (pair) p->kernel = r.f8 ? (const void *)linear_tile<2, true, false> : (const void *)linear_tile<2, false, false>;
@@ -1174,26 +1204,24 @@ void plan_split(const Rec &r, int sms, dnxcu_linear_plan *p) {
   a.BN = a.M >= 256 ? 256 : round_up(a.M, 16);
   a.mt = (a.M + a.BN - 1) / a.BN;
   a.nt = (a.N + 127) / 128;
-  // the split with the fewest steps on the busiest SM, the smaller one of equals
+  // Blocks up to the number of SMs, by powers of two (16 x 4096 x 4096: 10.6 us with 4 parts of c_in, 128 blocks; 12.1
+  // with 5, 13.5 with 8); twice that where every part is still 64 steps or more (64 x 8192 x 8192: 28.7 against 30.6 us).
   const long long tiles = (long long)a.mt * a.nt;
-  long long best = 0;
-  for (int s = 1; s <= 8 && s <= a.kb; ++s) {
-    const long long cost = (tiles * s + sms - 1) / sms * ((a.kb + s - 1) / s);
-    if (s == 1 || cost < best) {
-      best = cost;
-      a.split = s;
-    }
-  }
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= sms && s * 2 <= a.kb) s *= 2;
+  if (s < 8 && a.kb / s >= 64) s *= 2;
+  a.split = s;
   const uint32_t stage = 16384u + (uint32_t)a.BN * 128u, fixed = 1024u + SPLIT_FIXED;
   const int most = a.BN < a.M ? a.BN : a.M, per = (most + a.split - 1) / a.split;
   const uint32_t recv = (uint32_t)(a.split * per) * 512u;
-  // two blocks per SM where there are more blocks than SMs and shared memory leaves both some stages
+  // two blocks per SM where there are more blocks than SMs and shared memory leaves both some stages; six stages are
+  // as fast as twelve
   uint32_t room = kSmemLimit - fixed;
   if (tiles * a.split > sms && kSmemLimit / 2 - fixed - 1024u >= recv + 3 * stage) room = kSmemLimit / 2 - fixed - 1024u;
   a.overlay = recv + 3 * stage > room;
   int st = (int)((room - (a.overlay ? 0u : recv)) / stage);
   const int steps = (a.kb + a.split - 1) / a.split;
-  st = st > MAX_STAGES ? MAX_STAGES : st;
+  st = st > 6 ? 6 : st;
   a.stages = st > steps ? (steps > 2 ? steps : 2) : st;
   const uint32_t body = stage * (uint32_t)a.stages;
   p->smem = fixed + (a.overlay ? (body > recv ? body : recv) : body + recv);
@@ -1213,20 +1241,15 @@ int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxc
   if (v == DNXCU_LINEAR_ROWS || (v == DNXCU_LINEAR_ANY && a.M <= 16)) {
     p->block = dim3(ROWS_THREADS);
     const bool two = a.M > 8;
-    int mt = 1;
     if (v == DNXCU_LINEAR_ANY) {
       if (r.f8) p->kernel = two ? (const void *)linear_rows<true, 2, 1, 1, true> : (const void *)linear_rows<true, 1, 1, 1, true>;
       else p->kernel = two ? (const void *)linear_rows<false, 2, 1, 1, true> : (const void *)linear_rows<false, 1, 1, 1, true>;
-    } else if (r.f8 && (a.N + 15) / 16 > 3 * sms) {
-      // 8 bit weights and many channels: 32 per block, so that x is fetched half as often and blocks last longer
-      mt = 2;
-      p->kernel = two ? (const void *)linear_rows<true, 2, 2, 4, false> : (const void *)linear_rows<true, 1, 2, 4, false>;
     } else if (r.f8) {
-      p->kernel = two ? (const void *)linear_rows<true, 2, 1, 4, false> : (const void *)linear_rows<true, 1, 1, 4, false>;
+      p->kernel = two ? (const void *)linear_rows<true, 2, 1, 4, false> : (const void *)linear_rows<true, 1, 1, 8, false>;
     } else {
       p->kernel = two ? (const void *)linear_rows<false, 2, 1, 2, false> : (const void *)linear_rows<false, 1, 1, 4, false>;
     }
-    p->grid = dim3((unsigned)((a.N + 16 * mt - 1) / (16 * mt)));
+    p->grid = dim3((unsigned)((a.N + 15) / 16));
     return DNXCU_OK;
   }
   int st = init_device(p->device);
