@@ -80,6 +80,32 @@ bool rows_overlap(const RowSpan &a, const RowSpan &b);
 // Whether kernels on the current device may use the pointer: memory of this device, managed or registered host memory.
 bool on_current_device(const void *p);
 
+// Programmatic dependent launch.  A kernel launched with launch_dependent() may start while the kernels before it on the
+// stream are still finishing: its set-up (barriers, tensor memory, descriptor fetches) hides behind them.  It calls
+// pdl_wait() before its first access to memory that any of them may read or write, which returns when they are done and
+// their writes are visible.  pdl_release() lets the kernel behind it start in the same way.
+#ifdef __CUDACC__
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+inline cudaError_t launch_dependent(const void *kernel, dim3 grid, dim3 block, size_t smem, unsigned cluster, cudaStream_t s,
+                                    void **args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
 // SHA-256 (hex) of a byte string; used for variant identities and database keys.
 void sha256_hex(const void *data, size_t n, char out_hex[65]);
 

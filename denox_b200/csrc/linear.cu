@@ -118,16 +118,27 @@ __device__ __forceinline__ void bulk_group_commit() { asm volatile("cp.async.bul
 __device__ __forceinline__ void bulk_group_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_group_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// Operand tiles: rows of 128 bytes (64 binary16 or 128 e4m3 channels) with the 128 byte swizzle, K major.  Descriptor:
+// start address, 1024 bytes between groups of 8 rows, layout code 2.  A K step is 32 bytes for either type.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t operand_desc(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+// The MMA warp walks its loops as one warp, so that descriptors live in uniform registers; the lane with `leader` set
+// alone issues.  Descriptors are a constant high word and a low word.
 template <int CG, bool F8>
-__device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate,
+                                         uint32_t leader) {
 #define DNXCU_MMA(group, kind)                                                             \
   asm volatile(                                                                            \
       "{\n\t"                                                                              \
-      ".reg .pred p;\n\t"                                                                  \
-      "setp.ne.b32 p, %4, 0;\n\t"                                                          \
-      "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t"           \
+      ".reg .pred p, e;\n\t"                                                               \
+      ".reg .b64 da, db;\n\t"                                                              \
+      "mov.b64 da, {%1, %4};\n\t"                                                          \
+      "mov.b64 db, {%2, %4};\n\t"                                                          \
+      "setp.ne.b32 p, %5, 0;\n\t"                                                          \
+      "setp.ne.b32 e, %6, 0;\n\t"                                                          \
+      "@e tcgen05.mma.cta_group::" group ".kind::" kind " [%0], da, db, %3, p;\n\t"        \
       "}" ::"r"(d),                                                                        \
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)                                          \
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(accumulate), "r"(leader)         \
       : "memory")
   if (CG == 2 && F8) DNXCU_MMA("2", "f8f6f4");
   else if (CG == 2) DNXCU_MMA("2", "f16");
@@ -136,30 +147,47 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uin
 #undef DNXCU_MMA
 }
 // The `n` (1 to 4) steps of one stage, straight line code for each n: an MMA in a loop costs its thread about 200 cycles
-// of issue, one in straight line code about 60 (522240 rows, 32 to 32 channels: 22.0 us with a loop).
+// of issue, one in straight line code about 60 (522240 rows, 32 to 32 channels: 22.0 us with a loop, 20.6 without).
 template <int CG, bool F8, int N>
-__device__ __forceinline__ void mma_steps_n(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  mma_step<CG, F8>(d, a, b, idesc, accumulate);
+__device__ __forceinline__ void mma_steps_n(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+  mma_step<CG, F8>(d, a, b, idesc, accumulate, leader);
 #pragma unroll
-  for (int k = 1; k < N; ++k) mma_step<CG, F8>(d, a + 2 * k, b + 2 * k, idesc, 1u);
+  for (int k = 1; k < N; ++k) mma_step<CG, F8>(d, a + 2 * k, b + 2 * k, idesc, 1u, leader);
 }
 template <int CG, bool F8>
-__device__ __forceinline__ void mma_steps(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, int n) {
-  if (n == 4) mma_steps_n<CG, F8, 4>(d, a, b, idesc, accumulate);
-  else if (n == 2) mma_steps_n<CG, F8, 2>(d, a, b, idesc, accumulate);
-  else if (n == 1) mma_steps_n<CG, F8, 1>(d, a, b, idesc, accumulate);
-  else mma_steps_n<CG, F8, 3>(d, a, b, idesc, accumulate);
+__device__ __forceinline__ void mma_steps(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate, int n,
+                                          uint32_t leader) {
+  if (n == 4) mma_steps_n<CG, F8, 4>(d, a, b, idesc, accumulate, leader);
+  else if (n == 2) mma_steps_n<CG, F8, 2>(d, a, b, idesc, accumulate, leader);
+  else if (n == 1) mma_steps_n<CG, F8, 1>(d, a, b, idesc, accumulate, leader);
+  else mma_steps_n<CG, F8, 3>(d, a, b, idesc, accumulate, leader);
 }
 // Arrives on `bar` (of both blocks of a pair) when the MMAs issued so far are done.
 template <int CG>
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t leader) {
   if (CG == 2)
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "setp.ne.b32 e, %2, 0;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t"
+        "}" ::"r"(bar),
+        "h"((uint16_t)3), "r"(leader)
         : "memory");
   else
-    tc_commit(bar);
+    asm volatile(
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+        "}" ::"r"(bar),
+        "r"(leader)
+        : "memory");
+}
+// Bounded wait of a whole warp: the same answer in every lane.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code) {
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity) != 0)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
 }
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
@@ -185,12 +213,6 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// Operand tiles: rows of 128 bytes (64 binary16 or 128 e4m3 channels) with the 128 byte swizzle, K major.  Descriptor:
-// start address, 1024 bytes between groups of 8 rows, layout code 2.  A K step is 32 bytes for either type.
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
-  return ((uint64_t)kDescHi << 32) | (uint64_t)((addr >> 4) | (1u << 16));
-}
 // Instruction descriptor: 32 bit accumulators, both operands binary16 (0) or e4m3 (0 of the 8 bit kinds), K major.
 __device__ __forceinline__ uint32_t mma_idesc(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -205,7 +227,7 @@ __device__ __forceinline__ int k_steps(const LinArgs &g, int kb) {
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_BUFS = 4;  // accumulators in tensor memory
 constexpr int HDR_FULL = 0, HDR_EMPTY = 8 * MAX_STAGES, HDR_TFULL = 16 * MAX_STAGES, HDR_TEMPTY = HDR_TFULL + 8 * MAX_BUFS,
-              HDR_RES = HDR_TEMPTY + 8 * MAX_BUFS, HDR_WRES = HDR_RES + 128, HDR_TMEM = HDR_WRES + 8, HDR_ABORT = HDR_TMEM + 4;
+              HDR_RES = HDR_TEMPTY + 8 * MAX_BUFS, HDR_WRES = HDR_RES + 64, HDR_TMEM = HDR_WRES + 8, HDR_ABORT = HDR_TMEM + 4;
 static_assert((HDR_ABORT + 4) % 8 == 0 && HDR_ABORT + 12 <= 1024, "header layout");
 constexpr int HEADER = 1024;
 constexpr uint32_t kSmemLimit = 232448;
@@ -213,15 +235,14 @@ constexpr uint32_t kSmemLimit = 232448;
 __device__ __forceinline__ uint32_t aligned_base(const void *dyn) { return (smem_u32(dyn) + 1023u) & ~1023u; }
 
 // ---- TILE and ANY -----------------------------------------------------------
-// Warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7, 8-11, ... are one to four epilogue teams
-// that take turns; 2 or 4 accumulators rotate, so tiles are multiplied while the teams finish the ones before.  A team
-// needs about 2300 cycles for a tile of 32 channels whatever its products take (TMEM to registers to shared memory to the
-// copy engine, one after the other), so thin layers have four teams.  ANY: seven warps (0, 2, 3, 12-15) fetch with plain loads instead, each a whole stage, so that as many
+// Warps: 0 fetches operand tiles, 1 issues MMAs, 2 owns the tensor memory, 4-7 and 8-11 are two epilogue teams that take
+// turns (or one that takes all); 2 or 4 accumulators rotate, so tiles are multiplied while the teams finish the ones
+// before.  (Four teams, 96 registers each: 522240 rows, 32 to 32 channels 20.0 us, with two 19.1.)  ANY: seven warps (0, 2, 3, 12-15) fetch with plain loads instead, each a whole stage, so that as many
 // stages are on their way at any time.  Where all of c_out is one column of tiles and the weights are small (a pointwise layer over pixels), they are
 // fetched once per block and only rows of x stream.
-constexpr int PAIR_THREADS = 384, ONE_THREADS = 640, ANY_THREADS = 512;
+constexpr int TILE_THREADS = 384, ANY_THREADS = 512;
 constexpr int COLBUF = 512;              // per epilogue warp: bias and weight scale of 64 channels
-constexpr int TILE_FIXED = HEADER + 16 * COLBUF;
+constexpr int TILE_FIXED = HEADER + 8 * COLBUF;
 constexpr int STAGING = 4096;            // per epilogue warp: 32 rows x 64 channels of binary16
 
 struct TilePos {
@@ -328,7 +349,7 @@ constexpr int FETCHERS = 7;
 __device__ __forceinline__ int fetcher(int warp) { return warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : warp >= 12 ? warp - 9 : -1; }
 
 template <int CG, bool F8, bool ANY>
-__global__ void __launch_bounds__(ANY ? ANY_THREADS : CG == 2 ? PAIR_THREADS : ONE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
+__global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
   extern __shared__ uint8_t dyn[];
   const uint32_t base = aligned_base(dyn);
   uint8_t *hdr = dyn + (base - smem_u32(dyn));
@@ -348,7 +369,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : CG == 2 ? PAIR_THREADS : O
       mbar_init(base + HDR_FULL + 8 * i, 1);
       mbar_init(base + HDR_EMPTY + 8 * i, 1);
     }
-    for (int i = 0; i < 16; ++i) mbar_init(base + HDR_RES + 8 * i, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(base + HDR_RES + 8 * i, 1);
     mbar_init(base + HDR_WRES, ANY ? FETCHERS : 1);
     for (int i = 0; i < MAX_BUFS; ++i) {
       mbar_init(base + HDR_TFULL + 8 * i, 1);
@@ -369,6 +390,8 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : CG == 2 ? PAIR_THREADS : O
   if (CG == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(hdr + HDR_TMEM);
+  pdl_release();
+  pdl_wait();
 
   if (!ANY && warp == 0) {
     // ---- operand tiles by TMA; the pair's bytes are counted on the first block's barrier ----
@@ -440,33 +463,36 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : CG == 2 ? PAIR_THREADS : O
       }
     }
   } else if (warp == 1) {
-    // ---- MMA issue: one thread of the (first) block ----
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = mma_idesc(128 * CG, g.BN);
+    // ---- MMA issue: one warp of the (first) block ----
+    if (rank == 0) {
+      const uint32_t leader = lane == 0, idesc = mma_idesc(128 * CG, g.BN);
       const int last = k_steps<F8>(g, g.kb - 1);
+      const uint32_t a0 = operand_desc(stage0), a_step = stage_bytes >> 4, w0 = operand_desc(wres0), w_step = b_bytes >> 4;
       int s = 0, buf = 0;
-      uint32_t ph = 0, bph = 1;
-      bool ok = !g.w_res || mbar_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
+      uint32_t ph = 0, bph = 1, a = a0;
+      bool ok = !g.w_res || warp_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
       for (int t = first; ok && t < ntiles; t += step) {
         const uint32_t d = tmem + (uint32_t)(buf * g.BN);
-        ok = mbar_wait(base + HDR_TEMPTY + 8 * buf, bph, abort_flag, g.status, 14);
+        ok = warp_wait(base + HDR_TEMPTY + 8 * buf, bph, abort_flag, g.status, 14);
         if (!ok) break;
         tc_fence_after();
+        uint32_t w = w0;
         for (int kb = 0; kb < g.kb; ++kb) {
-          ok = mbar_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
+          ok = warp_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t at = stage0 + stage_bytes * (uint32_t)s;
-          const uint64_t a = operand_desc(at), b = operand_desc(g.w_res ? wres0 + (uint32_t)kb * b_bytes : at + 16384u);
-          mma_steps<CG, F8>(d, a, b, idesc, kb != 0, kb + 1 < g.kb ? 4 : last);
-          mma_commit<CG>(base + HDR_EMPTY + 8 * s);
+          mma_steps<CG, F8>(d, a, g.w_res ? w : a + (16384u >> 4), idesc, kb != 0, kb + 1 < g.kb ? 4 : last, leader);
+          mma_commit<CG>(base + HDR_EMPTY + 8 * s, leader);
+          w += w_step;
+          a += a_step;
           if (++s == g.stages) {
             s = 0;
+            a = a0;
             ph ^= 1;
           }
         }
         if (!ok) break;
-        mma_commit<CG>(base + HDR_TFULL + 8 * buf);
+        mma_commit<CG>(base + HDR_TFULL + 8 * buf, leader);
         if (++buf == g.bufs) {
           buf = 0;
           bph ^= 1;
@@ -675,10 +701,15 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
     }
     mbar_init(base + HDR_TFULL, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_map(&g.tm_w);
+    tma_prefetch_map(&g.tm_x);
+    pdl_release();
+    pdl_wait();
     // the first copies need nothing but the barriers: they are on their way while the rest is set up
     for (int i = 0; i < early; ++i) fetch(i, i);
   }
   if (warp == 2) tmem_alloc<1>(base + HDR_TMEM, cols);
+  pdl_wait();
   if (warp == 3)
     for (int i = lane; i < mine; i += 32) s_xs[i] = g.x_scale ? __ldg(g.x_scale + m0 + rank * per + i) : 1.0f;
   // the four channels this thread will finish, in every row it finishes
@@ -709,25 +740,23 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = mma_idesc(128, g.BN);
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int i = 0; i < nkb; ++i) {
-        ok = mbar_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t a = operand_desc(stage0 + stage_bytes * (uint32_t)s), b = a + (16384u >> 4);
-        mma_steps<1, F8>(tmem, a, b, idesc, i > 0, k_steps<F8>(g, step_of(i)));
-        mma_commit<1>(base + HDR_EMPTY + 8 * s);
-        if (++s == g.stages) {
-          s = 0;
-          ph ^= 1;
-        }
+    const uint32_t leader = lane == 0, idesc = mma_idesc(128, g.BN);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int i = 0; i < nkb; ++i) {
+      ok = warp_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t a = operand_desc(stage0 + stage_bytes * (uint32_t)s);
+      mma_steps<1, F8>(tmem, a, a + (16384u >> 4), idesc, i > 0, k_steps<F8>(g, step_of(i)), leader);
+      mma_commit<1>(base + HDR_EMPTY + 8 * s, leader);
+      if (++s == g.stages) {
+        s = 0;
+        ph ^= 1;
       }
-      if (ok) mma_commit<1>(base + HDR_TFULL);
     }
+    if (ok) mma_commit<1>(base + HDR_TFULL, leader);
   }
   __syncwarp();
   bool ok = mbar_wait(base + HDR_TFULL, 0, abort_flag, g.status, 13);
@@ -918,6 +947,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows(const __grid_cons
   }
   float acc[MT][NT][4] = {};
   int c = warp;
+  pdl_release();
+  pdl_wait();
   if (!ANY) {
     for (; c + 8 * (U - 1) < whole; c += 8 * U) {
       RowsChunk<F8, NT, MT> r[U];
@@ -1180,8 +1211,8 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   a.mt = (int)((a.M + 128ll * cg - 1) / (128 * cg));
   a.nt = (a.N + bn - 1) / bn;
   a.bufs = bn <= 128 ? 4 : 2;
-  // more epilogue teams where a tile's products are soon done; one, and more stages, where they take long
-  a.teams = any || pair ? (a.kb >= 16 && pair ? 1 : 2) : a.kb >= 16 ? 1 : bn > 128 ? 2 : 4;
+  // two epilogue teams where a tile's products are soon done; one, and more stages, where they take long
+  a.teams = a.kb >= 16 && !any ? 1 : 2;
   const uint32_t wbytes = (uint32_t)(bn / cg) * 128u;
   a.w_res = cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536;
   const uint32_t stage = 16384u + (a.w_res ? 0u : wbytes);
@@ -1192,7 +1223,7 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   const long long tiles = (long long)a.mt * a.nt;
   const int clusters = (int)(tiles < sms / cg ? tiles : sms / cg);
   p->grid = dim3((unsigned)(clusters * cg));
-  p->block = dim3(any ? ANY_THREADS : pair ? PAIR_THREADS : ONE_THREADS);
+  p->block = dim3(any ? ANY_THREADS : TILE_THREADS);
   p->cluster = (uint32_t)cg;
   if (any) p->kernel = r.f8 ? (const void *)linear_tile<1, true, true> : (const void *)linear_tile<1, false, true>;
   else if (pair) p->kernel = r.f8 ? (const void *)linear_tile<2, true, false> : (const void *)linear_tile<2, false, false>;
@@ -1340,23 +1371,12 @@ int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
 
 int launch(const dnxcu_linear_plan &p, cudaStream_t s) {
   if (p.relay_grid) {
-    if (p.f8) linear_relay<true><<<p.relay_grid, 256, 0, s>>>(p.relay);
-    else linear_relay<false><<<p.relay_grid, 256, 0, s>>>(p.relay);
-    DNXCU_CUDA(cudaGetLastError());
+    void *args[] = {const_cast<RelayArgs *>(&p.relay)};
+    DNXCU_CUDA(cudaLaunchKernel(p.f8 ? (const void *)linear_relay<true> : (const void *)linear_relay<false>, dim3(p.relay_grid), dim3(256),
+                                args, 0, s));
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = p.grid;
-  cfg.blockDim = p.block;
-  cfg.dynamicSmemBytes = p.smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
   void *args[] = {const_cast<LinArgs *>(&p.a)};
-  DNXCU_CUDA(cudaLaunchKernelExC(&cfg, p.kernel, args));
+  DNXCU_CUDA(launch_dependent(p.kernel, p.grid, p.block, p.smem, p.cluster, s, args));
   return DNXCU_OK;
 }
 

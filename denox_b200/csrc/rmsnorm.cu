@@ -323,8 +323,12 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
 constexpr unsigned kMaxGrid = 0x7fffffffu;
 
 template <int V, bool Q, bool RES>
-void launch_v(const NormArgs &g, cudaStream_t s) {
+cudaError_t launch_v(const NormArgs &g, cudaStream_t s) {
   const int nv = g.C / V;
+  const auto enqueue = [&](const void *kernel, unsigned grid, int threads, int lt = 0) {
+    void *args[] = {const_cast<NormArgs *>(&g), &lt};  // (only the warp form takes the second)
+    return cudaLaunchKernel(kernel, dim3(grid), dim3((unsigned)threads), args, 0, s);
+  };
   if (g.C <= 1024) {
     // the fewest lanes (a power of two) that hold the row in 8, 16 or 32 elements per thread, most rows per warp first
     const int e = g.C <= 256 ? 8 : g.C <= 512 ? 16 : 32;
@@ -333,10 +337,9 @@ void launch_v(const NormArgs &g, cudaStream_t s) {
     const long long per_block = (256 >> lt) * (32 / e);
     const long long blocks = (g.rows + per_block - 1) / per_block;
     const unsigned grid = (unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid);
-    if (e == 8) rmsnorm_warp<V, 8, Q, RES><<<grid, 256, 0, s>>>(g, lt);
-    else if (e == 16) rmsnorm_warp<V, 16, Q, RES><<<grid, 256, 0, s>>>(g, lt);
-    else rmsnorm_warp<V, 32, Q, RES><<<grid, 256, 0, s>>>(g, lt);
-    return;
+    if (e == 8) return enqueue((const void *)rmsnorm_warp<V, 8, Q, RES>, grid, 256, lt);
+    if (e == 16) return enqueue((const void *)rmsnorm_warp<V, 16, Q, RES>, grid, 256, lt);
+    return enqueue((const void *)rmsnorm_warp<V, 32, Q, RES>, grid, 256, lt);
   }
   const unsigned grid = (unsigned)(g.rows < kMaxGrid ? g.rows : kMaxGrid);
   const auto threads = [&](int e) {
@@ -344,18 +347,18 @@ void launch_v(const NormArgs &g, cudaStream_t s) {
     return (t + 31) / 32 * 32;
   };
   // few rows: as many threads per row as there are, for latency; many rows: 32 elements in flight per thread
-  if (g.rows <= 148 && threads(8) <= 1024) rmsnorm_block<V, 8, Q, RES><<<grid, threads(8), 0, s>>>(g);
-  else if (g.rows <= 148 && threads(16) <= 1024) rmsnorm_block<V, 16, Q, RES><<<grid, threads(16), 0, s>>>(g);
-  else if (threads(32) <= 1024) rmsnorm_block<V, 32, Q, RES><<<grid, threads(32), 0, s>>>(g);
-  else rmsnorm_loop<V, Q, RES><<<grid, 1024, 0, s>>>(g);
+  if (g.rows <= 148 && threads(8) <= 1024) return enqueue((const void *)rmsnorm_block<V, 8, Q, RES>, grid, threads(8));
+  if (g.rows <= 148 && threads(16) <= 1024) return enqueue((const void *)rmsnorm_block<V, 16, Q, RES>, grid, threads(16));
+  if (threads(32) <= 1024) return enqueue((const void *)rmsnorm_block<V, 32, Q, RES>, grid, threads(32));
+  return enqueue((const void *)rmsnorm_loop<V, Q, RES>, grid, 1024);
 }
 
 template <int V>
-void launch_q(const NormArgs &g, bool q, cudaStream_t s) {
-  if (q && g.residual) launch_v<V, true, true>(g, s);
-  else if (q) launch_v<V, true, false>(g, s);
-  else if (g.residual) launch_v<V, false, true>(g, s);
-  else launch_v<V, false, false>(g, s);
+cudaError_t launch_q(const NormArgs &g, bool q, cudaStream_t s) {
+  if (q && g.residual) return launch_v<V, true, true>(g, s);
+  if (q) return launch_v<V, true, false>(g, s);
+  if (g.residual) return launch_v<V, false, true>(g, s);
+  return launch_v<V, false, false>(g, s);
 }
 
 // The record with packed strides filled in, or why it cannot run.
@@ -454,11 +457,7 @@ int dnxcu_rmsnorm_launch(const dnxcu_rmsnorm *d, void *stream) {
     return !((uintptr_t)g.out & ob) && g.os % v == 0;
   };
   cudaStream_t s = (cudaStream_t)stream;
-  if (fits(8)) launch_q<8>(g, q, s);
-  else if (fits(4)) launch_q<4>(g, q, s);
-  else if (fits(2)) launch_q<2>(g, q, s);
-  else launch_q<1>(g, q, s);
-  DNXCU_CUDA(cudaGetLastError());
+  DNXCU_CUDA(fits(8) ? launch_q<8>(g, q, s) : fits(4) ? launch_q<4>(g, q, s) : fits(2) ? launch_q<2>(g, q, s) : launch_q<1>(g, q, s));
   return DNXCU_OK;
 }
 
