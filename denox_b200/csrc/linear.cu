@@ -1128,8 +1128,53 @@ bool fits_tc(const Rec &r) {
 bool fits_rows(const Rec &r) { return r.d.rows <= 16 && fits_tc(r) && !((long long)r.d.c_in * r.es & 15); }
 bool fits_split(const Rec &r) { return fits_tc(r) && (r.d.rows + 15) / 16 <= 65535; }
 
+int round_up(int v, int m) { return (v + m - 1) / m * m; }
+
+// Time models in microseconds on an otherwise idle B200, fitted to sweeps over 17 .. 8192 rows, 128 .. 16384 channels; they
+// only rank the choices.  `kb`: 128 byte steps of c_in.
+struct TileShape {
+  int bn, cg;  // output channels per tile; blocks that share it (128 rows each)
+  double us;
+};
+// A wave of tiles costs its steps, issue bound at 0.31 us up to 128 channels and growing with the operand bytes above, and
+// the epilogue that is not hidden; 512 x 4096 x 4096: 64 channels 45.4 us (two waves), 128 27.3, 256 33.5; 2048 x 2048 x 2048:
+// 128 29.4 (two waves), 256 20.8; 1024 x 4096 x 4096: 128 48.8, 256 35.2, pairs of 256 32.0.
+TileShape pick_tile(long long rows, int n, int kb, int sms, bool any) {
+  TileShape best{0, 1, 0.0};
+  const auto consider = [&](int bn, int cg) {
+    const long long tiles = (rows + 128 * cg - 1) / (128 * cg) * ((n + bn - 1) / bn), waves = (tiles * cg + sms - 1) / sms;
+    const double step = bn <= 128 ? 0.31 : cg == 2 ? 0.37 : 0.31 + (bn - 128) * 0.0006;
+    const double us = 5.0 + (double)waves * (kb * step + bn * 0.008);
+    if (!best.bn || us < best.us) best = {bn, cg, us};
+  };
+  const int most = any ? 128 : 256;
+  if (n <= most) consider(round_up(n, 16), 1);
+  for (int bn = 64; bn <= most && bn < n; bn += 64) consider(bn, 1);
+  if (!any && n > 192) consider(256, 2);
+  return best;
+}
+// c_in over blocks up to the number of SMs, by powers of two (16 x 4096 x 4096: 10.6 us with 4 parts, 128 blocks; 12.1 with
+// 5, 13.5 with 8); twice that where every part is still 64 steps or more (64 x 8192 x 8192: 28.7 against 30.6 us).
+struct SplitShape {
+  int bn, split;
+  double us;
+};
+SplitShape pick_split(long long rows, int n, int kb, int sms) {
+  SplitShape p{rows >= 256 ? 256 : round_up((int)rows, 16), 1, 0.0};
+  const long long tiles = (rows + p.bn - 1) / p.bn * ((n + 127) / 128);
+  while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= kb) p.split *= 2;
+  if (p.split < 8 && kb / p.split >= 64) p.split *= 2;
+  const double waves = (double)((tiles * p.split + sms - 1) / sms);
+  p.us = 4.0 + 0.03 * p.bn + waves * ((kb + p.split - 1) / p.split) * (0.34 + (p.bn > 128 ? (p.bn - 128) * 0.0012 : 0.0));
+  return p;
+}
+int aligned_variant(long long rows, int n, int kb, int sms) {
+  return rows <= 2048 && pick_split(rows, n, kb, sms).us < pick_tile(rows, n, kb, sms, false).us ? DNXCU_LINEAR_SPLIT : DNXCU_LINEAR_TILE;
+}
+int k_blocks(const Rec &r) { return (int)(((long long)r.d.c_in * r.es + 127) / 128); }
+
 // The variant that runs the record.
-int pick(const Rec &r) {
+int pick(const Rec &r, int sms) {
   switch (r.d.variant) {
     case DNXCU_LINEAR_ROWS: return fits_rows(r) ? (int)DNXCU_LINEAR_ROWS : (int)DNXCU_E_UNSUPPORTED;
     case DNXCU_LINEAR_SPLIT: return fits_split(r) ? (int)DNXCU_LINEAR_SPLIT : (int)DNXCU_E_UNSUPPORTED;
@@ -1139,7 +1184,7 @@ int pick(const Rec &r) {
   }
   if (!fits_tc(r)) return DNXCU_LINEAR_ANY;
   if (fits_rows(r)) return DNXCU_LINEAR_ROWS;
-  return r.d.rows <= 256 ? DNXCU_LINEAR_SPLIT : DNXCU_LINEAR_TILE;
+  return aligned_variant(r.d.rows, r.d.c_out, k_blocks(r), sms);
 }
 
 }  // namespace
@@ -1163,6 +1208,7 @@ namespace dnxcu {
 namespace {
 
 constexpr int kMaxDevices = 64;
+constexpr int kSmCount = 148;  // of a B200, for the calls that touch no device
 
 int sm_count(int dev) {
   static std::atomic<int> cache[kMaxDevices];
@@ -1187,20 +1233,10 @@ int init_device(int dev) {
   return DNXCU_OK;
 }
 
-int round_up(int v, int m) { return (v + m - 1) / m * m; }
-
 void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   LinArgs &a = p->a;
-  // a pair of blocks (256 rows) where there are enough rows and channels to fill the machine with such tiles
-  const long long m128 = (a.M + 127) / 128;
-  int bn = a.N <= 256 ? round_up(a.N, 16) : 256;
-  const bool pair = !any && bn == 256 && (m128 + 1) / 2 * ((a.N + 255) / 256) * 2 >= sms;
-  if (!pair) {
-    if (any) bn = bn > 128 ? 128 : bn;
-    while (bn > 64 && m128 * ((a.N + bn - 1) / bn) < sms) bn = bn > 128 ? 128 : 64;
-    if (a.N > bn && bn % 64) bn = round_up(bn, 64);
-  }
-  const int cg = pair ? 2 : 1;
+  const TileShape shape = pick_tile(a.M, a.N, a.kb, sms, any);
+  const int bn = shape.bn, cg = shape.cg;
   // The weights pass through L2 once per group of rows, so a group is as many rows as keep 36 MB of x (of 126 MB of L2)
   // in flight, 4 to 32 tiles.  8192 x 4096 x 16384 binary16, 16 tiles against 8: 335 against 604 MB from memory, 942
   // against 955 us under the power limit; 8192 x 8192 x 8192, where 16 tiles are 67 MB: 990 against 975 us.
@@ -1226,22 +1262,18 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   p->block = dim3(any ? ANY_THREADS : TILE_THREADS);
   p->cluster = (uint32_t)cg;
   if (any) p->kernel = r.f8 ? (const void *)linear_tile<1, true, true> : (const void *)linear_tile<1, false, true>;
-  else if (pair) p->kernel = r.f8 ? (const void *)linear_tile<2, true, false> : (const void *)linear_tile<2, false, false>;
+  else if (cg == 2) p->kernel = r.f8 ? (const void *)linear_tile<2, true, false> : (const void *)linear_tile<2, false, false>;
   else p->kernel = r.f8 ? (const void *)linear_tile<1, true, false> : (const void *)linear_tile<1, false, false>;
 }
 
 void plan_split(const Rec &r, int sms, dnxcu_linear_plan *p) {
   LinArgs &a = p->a;
-  a.BN = a.M >= 256 ? 256 : round_up(a.M, 16);
+  const SplitShape shape = pick_split(a.M, a.N, a.kb, sms);
+  a.BN = shape.bn;
+  a.split = shape.split;
   a.mt = (a.M + a.BN - 1) / a.BN;
   a.nt = (a.N + 127) / 128;
-  // Blocks up to the number of SMs, by powers of two (16 x 4096 x 4096: 10.6 us with 4 parts of c_in, 128 blocks; 12.1
-  // with 5, 13.5 with 8); twice that where every part is still 64 steps or more (64 x 8192 x 8192: 28.7 against 30.6 us).
   const long long tiles = (long long)a.mt * a.nt;
-  int s = 1;
-  while (s < 8 && tiles * s * 2 <= sms && s * 2 <= a.kb) s *= 2;
-  if (s < 8 && a.kb / s >= 64) s *= 2;
-  a.split = s;
   const uint32_t stage = 16384u + (uint32_t)a.BN * 128u, fixed = 1024u + SPLIT_FIXED;
   const int most = a.BN < a.M ? a.BN : a.M, per = (most + a.split - 1) / a.split;
   const uint32_t recv = (uint32_t)(a.split * per) * 512u;
@@ -1276,7 +1308,9 @@ int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxc
       if (r.f8) p->kernel = two ? (const void *)linear_rows<true, 2, 1, 1, true> : (const void *)linear_rows<true, 1, 1, 1, true>;
       else p->kernel = two ? (const void *)linear_rows<false, 2, 1, 1, true> : (const void *)linear_rows<false, 1, 1, 1, true>;
     } else if (r.f8) {
-      p->kernel = two ? (const void *)linear_rows<true, 2, 1, 4, false> : (const void *)linear_rows<true, 1, 1, 8, false>;
+      // (16 x 4096 x 12288: 15.1 us with four chunks on their way, 13.3 with two and more blocks per SM; x 4096: 6.3 and 6.6)
+      const void *k2 = (a.N + 15) / 16 > 2 * sms ? (const void *)linear_rows<true, 2, 1, 2, false> : (const void *)linear_rows<true, 2, 1, 4, false>;
+      p->kernel = two ? k2 : (const void *)linear_rows<true, 1, 1, 4, false>;
     } else {
       p->kernel = two ? (const void *)linear_rows<false, 2, 1, 2, false> : (const void *)linear_rows<false, 1, 1, 4, false>;
     }
@@ -1306,13 +1340,13 @@ int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxc
 // `keep`: the plan outlives this call and may hold scratch memory.
 int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
   const dnxcu_linear &d = r.d;
-  const int v = pick(r);
-  if (v < 0) return v;
   DNXCU_CUDA(cudaGetDevice(&p->device));
+  const int sms = sm_count(p->device);
+  const int v = pick(r, sms);
+  if (v < 0) return v;
   for (const void *q : {d.x, d.weights, (const void *)d.x_scale, (const void *)d.w_scale, d.bias, d.residual, (const void *)d.out,
                         (const void *)d.device_status})
     if (!on_current_device(q)) return DNXCU_E_BAD_ARG;
-  const int sms = sm_count(p->device);
   p->f8 = r.f8;
   LinArgs &a = p->a;
   memset(&a, 0, sizeof(a));
@@ -1330,7 +1364,7 @@ int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
   a.K = d.c_in;
   a.act = d.activation;
   a.alpha = d.leaky_alpha;
-  a.kb = (int)(((long long)d.c_in * r.es + 127) / 128);
+  a.kb = k_blocks(r);
   a.status = d.device_status;
   a.wait_limit = wait_limit_cycles();
   if (a.wait_limit < 2000000ull) a.wait_limit |= 1ull << 63;  // below about a millisecond: strict (see mbar_wait)
@@ -1360,7 +1394,7 @@ int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
       if (rx) a.xs = pitch;
       if (rw) a.ws = pitch;
       p->variant = v;
-      return plan_kernel(r, a.M <= 256 ? DNXCU_LINEAR_SPLIT : DNXCU_LINEAR_TILE, rx ? y.dst[0] : d.x, rw ? y.dst[1] : d.weights, sms, p);
+      return plan_kernel(r, aligned_variant(a.M, a.N, a.kb, sms), rx ? y.dst[0] : d.x, rw ? y.dst[1] : d.weights, sms, p);
     }
     cudaGetLastError();  // (no room: the kernel that fetches by plain loads needs none)
     p->scratch = nullptr;
@@ -1389,14 +1423,14 @@ int dnxcu_linear_validate(const dnxcu_linear *d) {
   Rec r;
   const int st = check(d, &r);
   if (st) return st;
-  const int v = pick(r);
+  const int v = pick(r, kSmCount);
   return v < 0 ? v : DNXCU_OK;
 }
 
 int dnxcu_linear_pick(const dnxcu_linear *d) {
   Rec r;
   const int st = check(d, &r);
-  return st ? st : pick(r);
+  return st ? st : pick(r, kSmCount);
 }
 
 int dnxcu_linear_launch(const dnxcu_linear *d, void *stream) {

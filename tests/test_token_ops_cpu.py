@@ -69,7 +69,8 @@ def test_linear_accepts_and_picks():
         return got
 
     assert pick(rows=1) == lib.LINEAR_ROWS
-    assert pick(rows=100) == lib.LINEAR_SPLIT
+    assert pick(rows=100, c_in=4096, c_out=4096) == lib.LINEAR_SPLIT and pick(rows=100) == lib.LINEAR_TILE
+    assert pick(rows=300, c_in=16384, c_out=1024) == lib.LINEAR_SPLIT and pick(rows=300, c_in=512, c_out=8192) == lib.LINEAR_TILE
     assert pick(rows=100000) == lib.LINEAR_TILE
     assert pick(rows=100000, dtype=lib.DT_E4M3) == lib.LINEAR_TILE
     assert pick(c_in=65) == lib.LINEAR_ANY and pick(x=X + 2) == lib.LINEAR_ANY and pick(weights=W + 8) == lib.LINEAR_ANY
