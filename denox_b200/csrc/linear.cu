@@ -34,6 +34,7 @@ struct LinArgs {
   int mt, nt;    // tiles along rows and output channels
   int kb;        // 128 byte wide steps along c_in
   int stages;
+  int per_stage; // tile: 128 byte steps per stage (1 or 2)
   int split;     // split: blocks per cluster
   int overlay;   // split: the received partial sums lie over the operand stages
   int teams;     // tile: epilogue teams
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(hdr + HDR_ABORT);
   const uint32_t b_rows = (uint32_t)g.BN / CG, b_bytes = b_rows * 128u;
-  const uint32_t stage_bytes = 16384u + (g.w_res ? 0u : b_bytes);
+  const uint32_t step_bytes = 16384u + (g.w_res ? 0u : b_bytes), stage_bytes = step_bytes * (uint32_t)g.per_stage;
   const uint32_t wres0 = base + TILE_FIXED, stage0 = wres0 + (g.w_res ? (uint32_t)g.kb * b_bytes : 0u);
   const uint32_t staging0 = stage0 + stage_bytes * (uint32_t)g.stages;
   const int ntiles = g.mt * g.nt, step = (int)gridDim.x / CG, first = (int)blockIdx.x / CG;
@@ -407,15 +408,18 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       for (int t = first; ok && t < ntiles; t += step) {
         const TilePos p = tile_pos(g, t);
         const int row_a = p.m * (128 * CG) + (int)rank * 128, row_b = p.n * g.BN + (int)(rank * b_rows);
-        for (int kb = 0; kb < g.kb; ++kb) {
+        for (int kb = 0; kb < g.kb;) {
           ok = mbar_wait(base + HDR_EMPTY + 8 * s, ph, abort_flag, g.status, 12);
           if (!ok) break;
           const uint32_t full = base + HDR_FULL + 8 * s;
-          if (rank == 0) mbar_expect_tx(full, stage_bytes * CG);
+          const int end = min(kb + g.per_stage, g.kb);
+          if (rank == 0) mbar_expect_tx(full, step_bytes * (uint32_t)(end - kb) * CG);
           const uint32_t bar = CG == 2 ? map_rank(full, 0) : full;
-          const uint32_t a = stage0 + stage_bytes * (uint32_t)s;
-          tma_load_2d<CG>(a, &g.tm_x, kb * (F8 ? 128 : 64), row_a, bar);
-          if (!g.w_res) tma_load_2d<CG>(a + 16384u, &g.tm_w, kb * (F8 ? 128 : 64), row_b, bar);
+          uint32_t a = stage0 + stage_bytes * (uint32_t)s;
+          for (; kb < end; ++kb, a += step_bytes) {
+            tma_load_2d<CG>(a, &g.tm_x, kb * (F8 ? 128 : 64), row_a, bar);
+            if (!g.w_res) tma_load_2d<CG>(a + 16384u, &g.tm_w, kb * (F8 ? 128 : 64), row_b, bar);
+          }
           if (++s == g.stages) {
             s = 0;
             ph ^= 1;
@@ -442,15 +446,17 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
     bool ok = pw < turns;
     for (int t = first; ok && t < ntiles; t += step) {
       const TilePos p = tile_pos(g, t);
-      for (int kb = 0; kb < g.kb; ++kb) {
+      for (int kb0 = 0; kb0 < g.kb; kb0 += g.per_stage) {
         if (turn == pw) {
           ok = mbar_wait(base + HDR_EMPTY + 8 * s, ph, abort_flag, g.status, 12);
           ok = __all_sync(0xffffffffu, ok);  // (the warp leaves the loop as one)
           if (!ok) break;
-          const uint32_t a = stage0 + stage_bytes * (uint32_t)s;
-          const int ks = k_steps<F8>(g, kb);
-          fill_tile<F8>(a, g.x, g.xs, (long long)p.m * 128, g.M, 128, ks, kb, kbytes, lane, 0, 1);
-          if (!g.w_res) fill_tile<F8>(a + 16384u, g.w, g.ws, (long long)p.n * g.BN, g.N, g.BN, ks, kb, kbytes, lane, 0, 1);
+          uint32_t a = stage0 + stage_bytes * (uint32_t)s;
+          for (int kb = kb0; kb < min(kb0 + g.per_stage, g.kb); ++kb, a += step_bytes) {
+            const int ks = k_steps<F8>(g, kb);
+            fill_tile<F8>(a, g.x, g.xs, (long long)p.m * 128, g.M, 128, ks, kb, kbytes, lane, 0, 1);
+            if (!g.w_res) fill_tile<F8>(a + 16384u, g.w, g.ws, (long long)p.n * g.BN, g.N, g.BN, ks, kb, kbytes, lane, 0, 1);
+          }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(base + HDR_FULL + 8 * s);
@@ -467,9 +473,10 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
     if (rank == 0) {
       const uint32_t leader = lane == 0, idesc = mma_idesc(128 * CG, g.BN);
       const int last = k_steps<F8>(g, g.kb - 1);
-      const uint32_t a0 = operand_desc(stage0), a_step = stage_bytes >> 4, w0 = operand_desc(wres0), w_step = b_bytes >> 4;
+      const uint32_t a0 = operand_desc(stage0), a_stage = stage_bytes >> 4, a_step = step_bytes >> 4;
+      const uint32_t w0 = operand_desc(wres0), w_step = b_bytes >> 4;
       int s = 0, buf = 0;
-      uint32_t ph = 0, bph = 1, a = a0;
+      uint32_t ph = 0, bph = 1, a_s = a0;
       bool ok = !g.w_res || warp_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
       for (int t = first; ok && t < ntiles; t += step) {
         const uint32_t d = tmem + (uint32_t)(buf * g.BN);
@@ -477,17 +484,27 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
         if (!ok) break;
         tc_fence_after();
         uint32_t w = w0;
-        for (int kb = 0; kb < g.kb; ++kb) {
+        for (int kb = 0; kb < g.kb;) {
           ok = warp_wait(base + HDR_FULL + 8 * s, ph, abort_flag, g.status, 11);
           if (!ok) break;
           tc_fence_after();
+          uint32_t a = a_s;
           mma_steps<CG, F8>(d, a, g.w_res ? w : a + (16384u >> 4), idesc, kb != 0, kb + 1 < g.kb ? 4 : last, leader);
-          mma_commit<CG>(base + HDR_EMPTY + 8 * s, leader);
           w += w_step;
-          a += a_step;
+          ++kb;
+          if (g.per_stage == 2 && kb < g.kb) {
+            a += a_step;
+            mma_steps<CG, F8>(d, a, g.w_res ? w : a + (16384u >> 4), idesc, 1u, kb + 1 < g.kb ? 4 : last, leader);
+            w += w_step;
+            ++kb;
+          }
+          // (the tile's last stage is handed back by the epilogue, which learns of it by the tile's own commit; ANY needs
+          // the stages back in order)
+          if (ANY || kb < g.kb) mma_commit<CG>(base + HDR_EMPTY + 8 * s, leader);
+          a_s += a_stage;
           if (++s == g.stages) {
             s = 0;
-            a = a0;
+            a_s = a0;
             ph ^= 1;
           }
         }
@@ -512,9 +529,12 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
     };
     uint32_t rph = 0, bph = 0;
     bool ok = true;
-    int turn = 0, buf = 0;
+    const int tile_stages = (g.kb + g.per_stage - 1) / g.per_stage % g.stages;
+    int turn = 0, buf = 0, s = 0;  // s: the stage after the tile's last one
     bool fresh = true;  // the team's first tile
     for (int t = first; ok && t < ntiles; t += step) {
+      s += tile_stages;
+      if (s >= g.stages) s -= g.stages;
       const int my_buf = buf;
       const uint32_t my_ph = bph;
       if (++buf == g.bufs) {
@@ -571,6 +591,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
+      if (!ANY && q == 0 && lane == 0) mbar_arrive(base + HDR_EMPTY + 8 * (s == 0 ? g.stages - 1 : s - 1));
       const uint32_t acc = tmem + (uint32_t)(my_buf * g.BN) + ((uint32_t)(q * 32) << 16);
       for (int c = 0; live && c < nc; c += 64) {
         if (c > 0) prepare(c);
@@ -1251,8 +1272,12 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   a.teams = a.kb >= 16 && !any ? 1 : 2;
   const uint32_t wbytes = (uint32_t)(bn / cg) * 128u;
   a.w_res = cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536;
-  const uint32_t stage = 16384u + (a.w_res ? 0u : wbytes);
   const uint32_t fixed = 1024u + TILE_FIXED + 4u * (uint32_t)a.teams * STAGING + (a.w_res ? (uint32_t)a.kb * wbytes : 0u);
+  // Two steps per stage where three such stages fit: half the waits and commits of the issuing warp, which is what bounds
+  // tiles of up to 128 channels.
+  uint32_t stage = 16384u + (a.w_res ? 0u : wbytes);
+  a.per_stage = a.kb > 1 && (kSmemLimit - fixed) / (2 * stage) >= 3 ? 2 : 1;
+  stage *= (uint32_t)a.per_stage;
   a.stages = (int)((kSmemLimit - fixed) / stage);
   if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
   p->smem = fixed + stage * (uint32_t)a.stages;
