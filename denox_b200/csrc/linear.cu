@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
   if (CG == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(hdr + HDR_TMEM);
-  pdl_release();
+  pdl_release();  // (after the allocation: blocks that wait for this kernel may hold tensor memory)
   pdl_wait();
 
   if (!ANY && warp == 0) {
@@ -724,7 +724,6 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_map(&g.tm_w);
     tma_prefetch_map(&g.tm_x);
-    pdl_release();
     pdl_wait();
     // the first copies need nothing but the barriers: they are on their way while the rest is set up
     for (int i = 0; i < early; ++i) fetch(i, i);
@@ -745,6 +744,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for before the first remote store)
   tc_fence_after();
+  // Only now, with its tensor memory in hand, does a block let the next kernel start: blocks of that one wait for this one
+  // while they hold theirs.
+  pdl_release();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(hdr + HDR_TMEM);
 
   if (warp == 0) {
@@ -1033,38 +1035,40 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) linear_rows(const __grid_cons
 
 // ---- operands that no copy engine takes, laid out anew -----------------------
 // Rows of any alignment to rows on 16 byte boundaries (what lies behind a row's end in its last piece is zero).  x and the
-// weights in one launch: pieces [0, first) are the first operand's.
+// weights in one launch: groups of rows [0, groups[0]) are the first operand's.
 struct RelayArgs {
   const uint8_t *src[2];
   uint8_t *dst[2];
-  long long stride[2], pitch[2], pieces[2];  // bytes per source row, per laid out row; 16 byte pieces in all
-  int rows[2], kbytes, per_row;              // pieces per row
+  long long stride[2], pitch;  // bytes per source row, per laid out row
+  int rows[2], groups[2];
+  int kbytes, per_row;         // 16 byte pieces per row
+  int per_group;               // rows per group: about 1024 pieces
+  uint32_t magic;              // 2^32 / per_row, rounded up (0 for 1): quotients of up to 2047 pieces are exact
 };
 template <bool F8>
 __global__ void __launch_bounds__(256) linear_relay(const RelayArgs g) {
   constexpr int B = 4;
-  const long long n = g.pieces[0] + g.pieces[1];
-  for (long long i0 = (long long)blockIdx.x * 256 * B + threadIdx.x; i0 < n; i0 += (long long)gridDim.x * 256 * B) {
-    PieceReq q[B];
-    uint8_t *to[B];
+  for (int grp = (int)blockIdx.x; grp < g.groups[0] + g.groups[1]; grp += (int)gridDim.x) {
+    const int o = grp >= g.groups[0], r0 = (o ? grp - g.groups[0] : grp) * g.per_group;
+    const int rows = min(g.per_group, g.rows[o] - r0), pieces = rows * g.per_row;
+    const uint8_t *src = g.src[o] + (long long)r0 * g.stride[o];
+    const uint8_t *end = g.src[o] + (long long)(g.rows[o] - 1) * g.stride[o] + g.kbytes;
+    uint8_t *dst = g.dst[o] + (long long)r0 * g.pitch;
+    const bool edge = r0 == 0 || r0 + rows == g.rows[o];
+    for (int i0 = threadIdx.x; i0 < pieces; i0 += 256 * B) {
+      PieceReq q[B];
+      long long to[B];
 #pragma unroll
-    for (int u = 0; u < B; ++u) {
-      long long i = i0 + 256 * u;
-      const bool in = i < n;
-      const int o = in && i >= g.pieces[0];
-      if (o) i -= g.pieces[0];
-      // (a 64 bit division only where the pieces of an operand do not fit in 32)
-      const uint32_t row = !in ? 0u : i >> 32 ? (uint32_t)((unsigned long long)i / (unsigned)g.per_row) : (uint32_t)i / (unsigned)g.per_row;
-      const int at = (int)(i - (long long)row * g.per_row) * 16;
-      const uint8_t *src = g.src[o];
-      to[u] = in ? g.dst[o] + row * g.pitch[o] + at : nullptr;
-      request_piece(q[u], src + row * g.stride[o] + at, in ? g.kbytes - at : 0, true, src,
-                    src + (g.rows[o] - 1) * g.stride[o] + g.kbytes);
-    }
+      for (int u = 0; u < B; ++u) {
+        const int i = i0 + 256 * u, r = rows == 1 ? 0 : g.magic ? (int)__umulhi((uint32_t)i, g.magic) : i, at = (i - r * g.per_row) * 16;
+        to[u] = (long long)r * g.pitch + at;
+        request_piece(q[u], src + (long long)r * g.stride[o] + at, i < pieces ? g.kbytes - at : 0, edge, g.src[o], end);
+      }
 #pragma unroll
-    for (int u = 0; u < B; ++u) {
-      const uint4 v = finish_piece<F8>(q[u]);
-      if (to[u]) *reinterpret_cast<uint4 *>(to[u]) = v;
+      for (int u = 0; u < B; ++u) {
+        const uint4 v = finish_piece<F8>(q[u]);
+        if (i0 + 256 * u < pieces) *reinterpret_cast<uint4 *>(dst + to[u]) = v;
+      }
     }
   }
 }
@@ -1362,6 +1366,19 @@ int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxc
   return DNXCU_OK;
 }
 
+// Device memory outside of any stream's order; a capture that this thread has under way is not disturbed.
+bool scratch_alloc(void **p, size_t bytes) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  const bool ok = cudaMalloc(p, bytes) == cudaSuccess;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (!ok) {
+    cudaGetLastError();
+    *p = nullptr;
+  }
+  return ok;
+}
+
 // `keep`: the plan outlives this call and may hold scratch memory.
 int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
   const dnxcu_linear &d = r.d;
@@ -1401,28 +1418,29 @@ int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
     const long long pitch = ((long long)a.K * r.es + 15) / 16 * 16;
     y.kbytes = a.K * r.es;
     y.per_row = (int)(pitch / 16);
+    y.per_group = y.per_row < 1024 ? 1024 / y.per_row : 1;
+    y.magic = y.per_row == 1 ? 0u : 0xffffffffu / (uint32_t)y.per_row + 1;
     y.src[0] = (const uint8_t *)d.x;
     y.src[1] = (const uint8_t *)d.weights;
     y.stride[0] = a.xs;
     y.stride[1] = a.ws;
     y.rows[0] = a.M;
     y.rows[1] = a.N;
-    y.pitch[0] = y.pitch[1] = pitch;
+    y.pitch = pitch;
+    if (rx) y.groups[0] = (a.M + y.per_group - 1) / y.per_group;
+    if (rw) y.groups[1] = (a.N + y.per_group - 1) / y.per_group;
     const size_t xb = rx ? (size_t)a.M * (size_t)pitch : 0, wb = rw ? (size_t)a.N * (size_t)pitch : 0;
-    y.pieces[0] = (long long)(xb / 16);
-    y.pieces[1] = (long long)(wb / 16);
-    if (cudaMalloc(&p->scratch, xb + wb) == cudaSuccess) {
+    if (scratch_alloc(&p->scratch, xb + wb)) {
       y.dst[0] = (uint8_t *)p->scratch;
       y.dst[1] = (uint8_t *)p->scratch + xb;
-      const long long blocks = (y.pieces[0] + y.pieces[1] + 1023) / 1024;
-      p->relay_grid = (unsigned)(blocks < 16ll * sms ? blocks : 16ll * sms);
+      const int groups = y.groups[0] + y.groups[1];
+      p->relay_grid = (unsigned)(groups < 16 * sms ? groups : 16 * sms);
       if (rx) a.xs = pitch;
       if (rw) a.ws = pitch;
       p->variant = v;
       return plan_kernel(r, aligned_variant(a.M, a.N, a.kb, sms), rx ? y.dst[0] : d.x, rw ? y.dst[1] : d.weights, sms, p);
     }
-    cudaGetLastError();  // (no room: the kernel that fetches by plain loads needs none)
-    p->scratch = nullptr;
+    // (no room: the kernel that fetches by plain loads needs none)
   }
   p->variant = v;
   return plan_kernel(r, v, d.x, d.weights, sms, p);
@@ -1497,7 +1515,10 @@ void dnxcu_linear_plan_destroy(dnxcu_linear_plan *p) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev != p->device) cudaSetDevice(p->device);
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (cudaFree(p->scratch) != cudaSuccess) cudaGetLastError();  // (waits for launches that still use it)
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (dev != p->device) cudaSetDevice(dev);
   }
   delete p;

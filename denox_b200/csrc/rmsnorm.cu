@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
   const int nv = g.C / V, t = threadIdx.x, nt = blockDim.x;
   int turn = 0;
   for (long long row = blockIdx.x; row < g.rows; row += gridDim.x, turn ^= 1) {
-    float ss = 0.0f;
+    double sum = 0.0;  // (a thread may add thousands of terms one after the other)
     uint32_t top = 0;
 #pragma unroll 4
     for (int vi = t; vi < nv; vi += nt) {
@@ -435,12 +435,15 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
       load_raw<V, RES>(g, row, vi * V, true, raw);
       sum_raw<V, RES>(raw, h);
       if (Q) load_weight<V>(g, vi * V, w);
+      float ss = 0.0f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         ss = fmaf(h[e], h[e], ss);
         if (Q) top = max(top, abs_bits(h[e] * w[e]));
       }
+      sum += ss;
     }
+    float ss = (float)sum;
     block_reduce(ss, top, turn);
     float scale = 0.0f;
     const float f = row_factor<Q>(g, ss, top, &scale);

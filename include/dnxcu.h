@@ -286,7 +286,7 @@ typedef enum dnxcu_activation {
  *   sum_out = h rounded to binary16                 (when sum_out is given)
  *   out = y rounded to binary16, or, with out_dtype DNXCU_DT_E4M3,
  *   out_scale[row] = max|y| / 448 (1 for a row of zeros), out = y / out_scale[row] rounded to e4m3.
- * Sums, statistics and y are held in 32 bits; y comes from the sum before it is rounded.  A row that holds a NaN
+ * Sums, statistics and y are held in 32 bits or more; y comes from the sum before it is rounded.  A row that holds a NaN
  * or an infinity has, with an 8 bit output, NaN in all of out and in out_scale; with a binary16 output what the
  * formula gives (other rows are untouched by it).
  * sum_out may be x or residual itself, and a binary16 out may be x or residual itself (same pointer and stride);
@@ -359,7 +359,7 @@ DNXCU_API int dnxcu_linear_launch(const dnxcu_linear *d, void *stream);
 /* The same planned once and launched many times, as dnxcu_plan_create does for a dispatch: checks, geometry and tensor
  * maps are worked out when the plan is made, on the device that is current then; launching it with another device
  * current is DNXCU_E_STATE.  With AUTO and operands that break the alignment of SPLIT and TILE, a plan for more than 16
- * rows holds scratch memory (allocated when it is made, so not during a stream capture) in which every launch first lays
+ * rows holds scratch memory (allocated when it is made) in which every launch first lays
  * those operands out on 16 byte boundaries: many times faster than the kernel that a direct launch of them gets.  The
  * caller owns the plan, keeps one per stream (or captured graph) that may launch concurrently, and destroys it after its
  * last launch. */

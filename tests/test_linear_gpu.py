@@ -302,3 +302,63 @@ def test_buffers_of_another_place_are_refused():
         p = C.c_void_p()
         assert lib.L.dnxcu_linear_plan_create(r, C.byref(p)) == lib.E_BAD_ARG
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "e4m3"])
+@pytest.mark.parametrize("variant,m,k,n", [("rows", 8, 8192, 64), ("split", 30, 8192, 128), ("tile", 200, 8192, 128), ("any", 40, 8191, 64),
+                                           ("tile", 2560, 1024, 3840)])
+def test_sums_are_held_in_32_bits(variant, m, k, n, dtype):
+    """The residual takes the rounded sum away: what is left shows the sum's last bits."""
+    t = torch.float16 if dtype == "f16" else torch.float8_e4m3fn
+    x, w = normal(91, m, k, dtype=torch.float32).to(torch.float8_e4m3fn), normal(92, n, k, dtype=torch.float32).to(torch.float8_e4m3fn)
+    x, w = x.to(torch.float32).to(t), w.to(torch.float32).to(t)
+    s, _ = reference(x, w)
+    ref, tol = reference(x, w, residual=(-s).half())
+    assert_within(run(x, w, residual=(-s).half(), variant=variant), ref, tol)
+
+
+def test_direct_call_in_a_capture_and_plans_made_during_one():
+    m, k, n = 40, 513, 200
+    x, w, _, _ = operands("f16", m, k, n, 95)
+    ref, tol = reference(x, w)
+    xd, wd = x.cuda(), w.cuda()
+    outs = [torch.zeros(m, n, dtype=torch.float16, device="cuda") for _ in range(2)]
+    descs = [lib.linear_desc(m, k, n, xd.data_ptr(), wd.data_ptr(), o.data_ptr()) for o in outs]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        st = torch.cuda.current_stream().cuda_stream
+        lib.linear(descs[0], st)
+        plan = lib.LinearPlan(descs[1])  # (unaligned: allocates its scratch)
+        plan.launch(st)
+    g.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        assert_within(o.cpu().double(), ref, tol)
+    del g
+    plan.close()
+
+
+@pytest.mark.parametrize("variant,m,k,n", [("split", 64, 2048, 512), ("tile", 300, 2048, 512), ("tile", 2560, 512, 3840), ("any", 100, 1001, 300)])
+def test_gives_up_cleanly_when_the_wait_limit_is_tiny(variant, m, k, n):
+    """With a limit of one microsecond ordinary waits run out: the launch returns, the status word may hold the wait's code,
+    and the device and the library are in order afterwards."""
+    x, w, _, _ = operands("f16", m, k, n, 97)
+    ref, tol = reference(x, w)
+    xd, wd = x.cuda(), w.cuda()
+    out, status = torch.zeros(m, n, dtype=torch.float16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    d = lib.linear_desc(m, k, n, xd.data_ptr(), wd.data_ptr(), out.data_ptr(), variant=VARIANTS[variant], device_status=status.data_ptr())
+    lib.check(lib.L.dnxcu_set_wait_limit_us(1))
+    try:
+        codes = []
+        for _ in range(3):
+            lib.linear(d)
+            torch.cuda.synchronize()
+            codes.append(int(status))
+            status.zero_()
+    finally:
+        lib.check(lib.L.dnxcu_set_wait_limit_us(0))
+    assert all(c == 0 or 11 <= c <= 15 for c in codes), codes
+    lib.linear(d)
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    assert_within(out.cpu().double(), ref, tol)

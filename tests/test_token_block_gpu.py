@@ -1,0 +1,81 @@
+"""The operators together, as a residual block runs them: norm with the residual's addition to 8 bits, a widening layer on
+the 8 bit rows, a narrowing layer that adds the residual stream back, and the next block's norm on it — one stream, one
+graph.  Every stage is held against its formula in 64 bits on what the stage before it gave."""
+import math
+
+import pytest
+import torch
+
+from denox_b200 import lib
+from test_linear_gpu import reference
+from test_rmsnorm_gpu import EPS, check_out, reference as norm_reference
+from token_util import assert_within, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def e4m3_weights(seed, n, k):
+    w = normal(seed, n, k, dtype=torch.float32, scale=1 / math.sqrt(k))
+    s = w.abs().amax(1) / 448.0
+    return (w / s[:, None]).to(torch.float8_e4m3fn).cuda(), s.cuda()
+
+
+@pytest.mark.parametrize("rows,c,wide", [(1, 256, 1024), (9, 512, 1536), (77, 384, 1000), (600, 1024, 4096), (1088 * 24, 64, 96), (130, 33, 65)])
+def test_block(rows, c, wide):
+    half = dict(dtype=torch.float16, device="cuda")
+    x, stream = normal(1, rows, c).cuda(), normal(2, rows, c).cuda()
+    g1, g2 = (1.0 + normal(3, c, dtype=torch.float32, scale=0.2)).half().cuda(), normal(4, c).cuda()
+    w1, s1 = e4m3_weights(5, wide, c)
+    w2, b1, b2 = normal(6, c, wide, scale=1 / math.sqrt(wide)).cuda(), normal(7, wide).cuda(), normal(8, c).cuda()
+    residual = torch.empty(rows, c, **half)
+    q, qs = torch.empty(rows, c, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(rows, dtype=torch.float32, device="cuda")
+    mid, out = torch.empty(rows, wide, **half), torch.empty(rows, c, **half)
+    p = lambda t: t.data_ptr()
+    norm1 = lib.rmsnorm_desc(rows, c, p(x), p(q), lib.DT_E4M3, EPS, p(residual), p(g1), p(residual), p(qs))
+    up = lib.LinearPlan(lib.linear_desc(rows, c, wide, p(q), p(w1), p(mid), lib.DT_E4M3, lib.ACT_SILU, x_scale=p(qs), w_scale=p(s1), bias=p(b1)))
+    down = lib.LinearPlan(lib.linear_desc(rows, wide, c, p(mid), p(w2), p(residual), bias=p(b2), residual=p(residual)))
+    norm2 = lib.rmsnorm_desc(rows, c, p(residual), p(out), eps=EPS, weight=p(g2))
+
+    def block(st):
+        lib.rmsnorm(norm1, st)
+        up.launch(st)
+        down.launch(st)
+        lib.rmsnorm(norm2, st)
+
+    # stage by stage
+    residual.copy_(stream)
+    lib.rmsnorm(norm1)
+    torch.cuda.synchronize()
+    h, y = norm_reference(x.cpu(), stream.cpu(), g1.cpu())
+    check_out(q.float().cpu().double(), qs.cpu().double(), y)
+    after_add = residual.clone()
+    up.launch()
+    torch.cuda.synchronize()
+    ref, tol = reference(q, w1, qs, s1, b1, act="silu")
+    assert_within(mid.cpu().double(), ref, tol, "up")
+    down.launch()
+    torch.cuda.synchronize()
+    ref, tol = reference(mid, w2, bias=b2, residual=after_add)
+    assert_within(residual.cpu().double(), ref, tol, "down")
+    lib.rmsnorm(norm2)
+    torch.cuda.synchronize()
+    check_out(out.cpu().double(), None, norm_reference(residual.cpu(), None, g2.cpu())[1])
+    want = out.clone(), residual.clone()
+    # at once, and replayed: the same bits
+    for _ in range(3):
+        residual.copy_(stream)
+        block(0)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0]) and torch.equal(residual, want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        block(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        residual.copy_(stream)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(residual, want[1])
+    del graph
+    up.close()
+    down.close()
