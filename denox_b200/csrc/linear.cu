@@ -42,6 +42,7 @@ struct LinArgs {
   int w_res;     // tile: the weights of the (one) column of tiles stay in shared memory
   int group;     // tile: tiles along the rows that are walked together
   int out_tma, res_tma;
+  int out_pack, res_pack;  // tile: packed rows of at most 64 channels: 32 of them are one piece of memory on a 16 byte boundary
   int *status;
   unsigned long long wait_limit;
 };
@@ -349,7 +350,35 @@ __device__ __forceinline__ void fill_tile(uint32_t dst, const uint8_t *op, long 
 constexpr int FETCHERS = 7;
 __device__ __forceinline__ int fetcher(int warp) { return warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : warp >= 12 ? warp - 9 : -1; }
 
-template <int CG, bool F8, bool ANY>
+// A warp's 32 staged rows (swizzled, 128 bytes apart) of `n` <= 64 channels from or to 32 packed rows, by 16 byte accesses.
+__device__ __forceinline__ __half *staged_at(uint8_t *stg, int r, int j) {
+  return reinterpret_cast<__half *>(stg + r * 128 + ((((j >> 3) ^ (r & 7)) << 4) | ((j & 7) << 1)));
+}
+template <bool OUT>
+__device__ __forceinline__ void copy_packed(uint8_t *stg, __half *rows, int n, int lane) {
+  union {
+    uint4 v;
+    __half h[8];
+  } a;
+  for (int i = lane; i < 4 * n; i += 32) {
+    int r = 8 * i / n, j = 8 * i - r * n;
+    if (!OUT) a.v = reinterpret_cast<const uint4 *>(rows)[i];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (OUT) a.h[e] = *staged_at(stg, r, j);
+      else *staged_at(stg, r, j) = a.h[e];
+      if (++j == n) {
+        j = 0;
+        ++r;
+      }
+    }
+    if (OUT) reinterpret_cast<uint4 *>(rows)[i] = a.v;
+  }
+}
+
+// NARROW: rows of out or of the residual may be ones that no tensor map takes; a kernel of its own, because the code for
+// them costs the others registers (frame 96 -> 64: 106 us without it, up to 129 with).
+template <int CG, bool F8, bool ANY, bool NARROW>
 __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
   extern __shared__ uint8_t dyn[];
   const uint32_t base = aligned_base(dyn);
@@ -525,7 +554,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
     const uint32_t rbar = base + HDR_RES + 8 * ew;
     const uint32_t my = stg + (uint32_t)lane * 128u;
     const auto staged = [&](int r, int j) {  // channel j of row r in the staging tile
-      return reinterpret_cast<__half *>(stg_p + r * 128 + ((((j >> 3) ^ (r & 7)) << 4) | ((j & 7) << 1)));
+      return staged_at(stg_p, r, j);
     };
     uint32_t rph = 0, bph = 0;
     bool ok = true;
@@ -565,7 +594,10 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
             mbar_expect_tx(rbar, STAGING);
             tma_load_2d<1>(stg, &g.tm_res, n0 + c, (int)row0, rbar);
           }
-        } else if (g.res) {
+        } else if (NARROW && g.res_pack && row0 + 32 <= g.M) {
+          copy_packed<false>(stg_p, const_cast<__half *>(g.res) + row0 * g.N, g.N, lane);
+          __syncwarp();
+        } else if (NARROW && g.res) {
           // (rows that no tensor map takes: 2 byte loads, 32 of them on their way)
 #pragma unroll
           for (int r0 = 0; r0 < 32; r0 += 16) {
@@ -636,13 +668,17 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
           }
         }
         // (a store through the tensor map writes whole 16 byte pieces: not for a row that ends inside one)
-        if (g.out_tma && (c + 64 <= nc || (g.N & 7) == 0)) {
+        if (!NARROW || (g.out_tma && (c + 64 <= nc || (g.N & 7) == 0))) {
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
             tma_store_2d(&g.tm_out, stg, n0 + c, (int)row0);
             bulk_group_commit();
           }
+        } else if (g.out_pack && row0 + 32 <= g.M) {
+          __syncwarp();
+          copy_packed<true>(stg_p, g.out + row0 * g.N, g.N, lane);
+          fence_proxy_async();
         } else {
           __syncwarp();
 #pragma unroll 8
@@ -1245,14 +1281,15 @@ int sm_count(int dev) {
   return n;
 }
 
+#define TILE_KERNEL(cg, f8, any, narrow) (const void *)linear_tile<cg, f8, any, narrow>
 // Shared memory opt-in of every kernel, once per device.
 int init_device(int dev) {
   static std::atomic<int> done[kMaxDevices];
   if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return DNXCU_OK;
-  const void *k[] = {(const void *)linear_tile<1, false, false>, (const void *)linear_tile<1, true, false>,
-                     (const void *)linear_tile<2, false, false>, (const void *)linear_tile<2, true, false>,
-                     (const void *)linear_tile<1, false, true>,  (const void *)linear_tile<1, true, true>,
-                     (const void *)linear_split<false>,          (const void *)linear_split<true>};
+  const void *k[] = {TILE_KERNEL(1, false, false, false), TILE_KERNEL(1, true, false, false), TILE_KERNEL(2, false, false, false),
+                     TILE_KERNEL(2, true, false, false),  TILE_KERNEL(1, false, false, true), TILE_KERNEL(1, true, false, true),
+                     TILE_KERNEL(2, false, false, true),  TILE_KERNEL(2, true, false, true),  TILE_KERNEL(1, false, true, true),
+                     TILE_KERNEL(1, true, true, true),    (const void *)linear_split<false>,  (const void *)linear_split<true>};
   for (const void *f : k) DNXCU_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit));
   if (dev < kMaxDevices) done[dev].store(1, std::memory_order_release);
   return DNXCU_OK;
@@ -1273,7 +1310,9 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   a.nt = (a.N + bn - 1) / bn;
   a.bufs = bn <= 128 ? 4 : 2;
   // two epilogue teams where a tile's products are soon done; one, and more stages, where they take long
-  a.teams = a.kb >= 16 && !any ? 1 : 2;
+  // or where the rows of out or of the residual take 2 byte accesses (8192 x 1024 x 1023 with residual: 76 us with one).
+  const bool narrow = !mappable(r.d.out, a.os * 2) || (r.d.residual && !mappable(r.d.residual, a.rs * 2));
+  a.teams = a.kb >= 16 && !any && !(narrow && a.kb < 32 && (long long)a.mt * a.nt > sms / cg) ? 1 : 2;
   const uint32_t wbytes = (uint32_t)(bn / cg) * 128u;
   a.w_res = cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536;
   const uint32_t fixed = 1024u + TILE_FIXED + 4u * (uint32_t)a.teams * STAGING + (a.w_res ? (uint32_t)a.kb * wbytes : 0u);
@@ -1290,9 +1329,12 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   p->grid = dim3((unsigned)(clusters * cg));
   p->block = dim3(any ? ANY_THREADS : TILE_THREADS);
   p->cluster = (uint32_t)cg;
-  if (any) p->kernel = r.f8 ? (const void *)linear_tile<1, true, true> : (const void *)linear_tile<1, false, true>;
-  else if (cg == 2) p->kernel = r.f8 ? (const void *)linear_tile<2, true, false> : (const void *)linear_tile<2, false, false>;
-  else p->kernel = r.f8 ? (const void *)linear_tile<1, true, false> : (const void *)linear_tile<1, false, false>;
+  const bool tail = narrow || (a.N & 7);  // (a row that ends inside 16 bytes: see the store)
+  if (any) p->kernel = r.f8 ? TILE_KERNEL(1, true, true, true) : TILE_KERNEL(1, false, true, true);
+  else if (cg == 2 && tail) p->kernel = r.f8 ? TILE_KERNEL(2, true, false, true) : TILE_KERNEL(2, false, false, true);
+  else if (cg == 2) p->kernel = r.f8 ? TILE_KERNEL(2, true, false, false) : TILE_KERNEL(2, false, false, false);
+  else if (tail) p->kernel = r.f8 ? TILE_KERNEL(1, true, false, true) : TILE_KERNEL(1, false, false, true);
+  else p->kernel = r.f8 ? TILE_KERNEL(1, true, false, false) : TILE_KERNEL(1, false, false, false);
 }
 
 void plan_split(const Rec &r, int sms, dnxcu_linear_plan *p) {
@@ -1361,6 +1403,8 @@ int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxc
   }
   a.out_tma = mappable(d.out, a.os * 2);
   a.res_tma = d.residual && mappable(d.residual, a.rs * 2);
+  a.out_pack = a.N <= 64 && a.os == a.N && !((uintptr_t)d.out & 15);
+  a.res_pack = d.residual && a.N <= 64 && a.rs == a.N && !((uintptr_t)d.residual & 15);
   if (a.out_tma && (st = matrix_map(&a.tm_out, d.out, false, a.M, a.N, a.os * 2, 32))) return st;
   if (a.res_tma && (st = matrix_map(&a.tm_res, d.residual, false, a.M, a.N, a.rs * 2, 32))) return st;
   return DNXCU_OK;

@@ -110,7 +110,7 @@ SIZES = [("rows", 1, 16, 1), ("rows", 1, 64, 16), ("rows", 2, 4096, 33), ("rows"
          ("split", 1, 16, 8), ("split", 1, 4096, 256), ("split", 16, 128, 128), ("split", 17, 160, 129), ("split", 100, 2048, 1000),
          ("split", 128, 272, 127), ("split", 250, 1024, 256), ("split", 257, 64, 300), ("split", 600, 528, 96),
          ("tile", 1, 16, 8), ("tile", 127, 64, 64), ("tile", 128, 128, 128), ("tile", 129, 144, 136), ("tile", 300, 80, 16),
-         ("tile", 1000, 208, 96), ("tile", 513, 1024, 999), ("tile", 700, 32, 40), ("tile", 2048, 512, 4736), ("tile", 5000, 256, 2305),
+         ("tile", 1000, 208, 96), ("tile", 513, 1024, 999), ("tile", 700, 32, 40), ("tile", 1000, 64, 33), ("tile", 1, 16, 63), ("tile", 333, 48, 1), ("tile", 20000, 64, 50), ("tile", 2048, 512, 4736), ("tile", 5000, 256, 2305),
          ("any", 1, 1, 1), ("any", 3, 9, 5), ("any", 1000, 9, 32), ("any", 129, 65, 127), ("any", 257, 1001, 129), ("any", 130, 130, 300),
          ("auto", 1, 4096, 4096), ("auto", 12, 3000, 777), ("auto", 64, 77, 77), ("auto", 5, 8, 3), ("auto", 4099, 1024, 1024)]
 
@@ -176,7 +176,7 @@ def test_strides(variant, dtype):
 
 
 @pytest.mark.parametrize("variant,m,k,n", [("rows", 4, 128, 72), ("split", 100, 128, 200), ("tile", 400, 128, 200), ("tile", 300, 64, 99),
-                                           ("any", 100, 77, 99)])
+                                           ("tile", 1001, 64, 37), ("any", 100, 77, 99), ("any", 300, 33, 33)])
 def test_residual_in_place(variant, m, k, n):
     x, w, _, _ = operands("f16", m, k, n, 31)
     r = normal(33, m, n)
