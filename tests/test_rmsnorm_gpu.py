@@ -60,7 +60,8 @@ def run(x, residual=None, weight=None, q=False, keep_sum=False, eps=EPS, strides
 
 SIZES = [(1, 1), (3, 2), (5, 9), (1000, 32), (77, 96), (129, 255), (33, 256), (19, 264), (7, 513), (9, 1000), (6, 1024),
          (3, 1025), (2, 4096), (1, 4096), (150, 2056), (4, 5001), (160, 5001), (2, 8191), (2, 16384), (149, 8200), (1, 32768),
-         (2, 33001), (1, 70001), (150, 40000)]
+         (2, 33001), (1, 70001), (150, 40000), (1000, 29), (3000, 3), (4100, 1), (2049, 2), (700, 130), (65, 254), (16, 255),
+         (17, 255), (5000, 7)]
 
 
 @pytest.mark.parametrize("q", [False, True], ids=["f16", "e4m3"])
@@ -105,7 +106,7 @@ def test_strides_and_alignment(strides, offsets, q, wide):
     assert_within(s, h, h.abs() * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25, "sum")
 
 
-@pytest.mark.parametrize("rows,c", [(9, 48), (7, 1000), (3, 4096), (2, 5001), (2, 40001)])
+@pytest.mark.parametrize("rows,c", [(9, 48), (300, 27), (7, 1000), (3, 4096), (2, 5001), (2, 40001)])
 def test_in_place(rows, c):
     """The sum over the residual and the output over x, as a block of layers keeps its buffers."""
     x, r, w = normal(10, rows, c), normal(11, rows, c), normal(12, c)
@@ -117,7 +118,7 @@ def test_in_place(rows, c):
     assert_within(mr.check(), h, h.abs() * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25, "sum")
 
 
-@pytest.mark.parametrize("c", [24, 640, 4096, 5001, 40001])
+@pytest.mark.parametrize("c", [24, 37, 640, 4096, 5001, 40001])
 def test_rows_that_are_not_finite_or_zero(c):
     """NaN, infinity, zeros, the type's lowest value and its smallest, each in a row of its own; other rows untouched."""
     low = torch.finfo(torch.float16).min
