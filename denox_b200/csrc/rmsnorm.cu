@@ -10,7 +10,8 @@
 // The maximum is taken on the absolute values' bit patterns, whose unsigned order is the values' order with NaN
 // above infinity: a row that is not finite shows in it, and one integer `redux` does a warp's.
 //
-// Bound by bytes.  Six forms, by the row's length and by what the alignment allows (V elements per access, 16 bytes
+// Bound by bytes: 16384 rows of 4096 with residual to e4m3 72.5 us (6.5 TB/s), 2088960 rows of 32 43.8 us (6.1 TB/s).  Six
+// forms, by the row's length and by what the alignment allows (V elements per access, 16 bytes
 // where every pointer and stride is a multiple of that):
 //   warp form  rows of at most 1024 channels: a power of two of lanes per row, several rows per warp; every thread
 //              has 32 elements in flight whatever the row's length (U rows of E elements, U * E = 32);

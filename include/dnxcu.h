@@ -263,7 +263,9 @@ DNXCU_API int dnxcu_conv3x3_pool_static(const void *in, int height, int width, i
  *  - launches are stream ordered, never synchronise, allocate nothing, keep
  *    nothing between calls and may be captured into a graph; the stream
  *    belongs to the current device, which also holds every buffer;
- *  - results do not depend on timing: the same call gives the same bits.
+ *  - results do not depend on timing: the same call gives the same bits (a
+ *    plan and a direct launch of unaligned operands, or calls of other row
+ *    counts, may add in another order).
  * Limits: rows <= 2^31 - 1, channels <= 2^24, row strides < 2^35 elements.
  * ---------------------------------------------------------------------- */
 typedef enum dnxcu_dtype {
