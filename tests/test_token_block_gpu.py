@@ -79,3 +79,45 @@ def test_block(rows, c, wide):
     del graph
     up.close()
     down.close()
+
+
+def test_every_kernel_at_once_on_three_streams():
+    """Chains of all the kernels (row, split, single and paired tiles, unaligned plans, norms) on three streams at once: the
+    bits of each alone."""
+    half = dict(dtype=torch.float16, device="cuda")
+    p = lambda t: t.data_ptr()
+    shapes = [(1, 512, 700), (40, 4096, 512), (200, 256, 1024), (2560, 512, 3840), (300, 257, 129), (5000, 32, 48)]
+    keep, chains = [], []
+    for k in range(3):
+        chain = []
+        for i, (m, c, n) in enumerate(shapes[k:] + shapes[:k]):
+            x, w, b = normal(10 * i + k, m, c).cuda(), normal(10 * i + k + 5, n, c, scale=1 / math.sqrt(c)).cuda(), normal(i, n).cuda()
+            mid, out, scale = torch.empty(m, n, **half), torch.empty(m, n, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(m, device="cuda")
+            plan = lib.LinearPlan(lib.linear_desc(m, c, n, p(x), p(w), p(mid), bias=p(b), activation=lib.ACT_GELU))
+            norm = lib.rmsnorm_desc(m, n, p(mid), p(out), lib.DT_E4M3, EPS, out_scale=p(scale))
+            keep += [x, w, b]
+            chain.append((plan, norm, mid, out, scale))
+        chains.append(chain)
+
+    def launch(chain, st):
+        for plan, norm, *_ in chain:
+            plan.launch(st)
+            lib.rmsnorm(norm, st)
+
+    bits = lambda chain: [t.view(torch.uint8).clone() for c in chain for t in c[2:]]
+    torch.cuda.synchronize()
+    want = []
+    for chain in chains:
+        launch(chain, 0)
+        torch.cuda.synchronize()
+        want.append(bits(chain))
+    streams = [torch.cuda.Stream() for _ in chains]
+    for _ in range(15):
+        for chain, st in zip(chains, streams):
+            launch(chain, st.cuda_stream)
+    torch.cuda.synchronize()
+    for chain, w in zip(chains, want):
+        assert all(torch.equal(a, b) for a, b in zip(bits(chain), w))
+    for chain in chains:
+        for plan, *_ in chain:
+            plan.close()
