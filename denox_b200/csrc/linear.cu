@@ -11,7 +11,8 @@
 //   linear_tile   (TILE, ANY)  persistent tcgen05 tiles of 128 rows per block, or of 256 rows over a pair of blocks
 //                              (cta_group::2); ANY fills the same shared memory tiles with plain loads.  8192 x 4096 x
 //                              16384 binary16 with gelu: 750 to 890 us by clock (1.24 to 1.47 PFLOP/s), tensor pipe
-//                              88 % busy, bound by the power limit; 2088960 rows of 96 to 64: 105 us, 6.35 TB/s.
+//                              88 % busy, bound by the power limit; 2088960 rows of 96 to 64: 105 us, 6.35 TB/s;
+//                              522240 rows of 9 to 32 (GROUPED): 21 us.
 #include "internal.h"
 #include "tc_ptx.h"
 #include <cuda.h>
@@ -45,6 +46,7 @@ struct LinArgs {
   int teams;     // tile: epilogue teams
   int bufs;      // tile: accumulators
   int w_res;     // tile: the weights of the (one) column of tiles stay in shared memory
+  int gr, n1, k1;  // tile: rows taken together as one (see GROUPED), and the channels of a single one; gr = 1: none
   int group;     // tile: tiles along the rows that are walked together
   int out_tma, res_tma;
   int out_pack, res_pack;  // tile: packed rows of at most 64 channels: 32 of them are one piece of memory on a 16 byte boundary
@@ -355,6 +357,31 @@ __device__ __forceinline__ void fill_tile(uint32_t dst, const uint8_t *op, long 
 constexpr int FETCHERS = 7;
 __device__ __forceinline__ int fetcher(int warp) { return warp == 0 ? 0 : warp == 2 ? 1 : warp == 3 ? 2 : warp >= 12 ? warp - 9 : -1; }
 
+// GROUPED: thin layers over packed rows (pixels).  `gr` rows side by side are one row of gr * c_in channels, whose product
+// with the block diagonal of gr copies of the weights is the gr output rows side by side.  The zeros cost multiplications
+// that nothing waits for; in return tiles are wide (a tile of 32 channels takes the epilogue nearly as long as one of 128),
+// and rows off 16 byte boundaries become rows on them.  The block diagonal is put together in shared memory, once per block.
+template <bool F8>
+__device__ __forceinline__ void fill_grouped(uint32_t wres, uint32_t step_bytes, const LinArgs &g) {
+  constexpr int E = F8 ? 16 : 8;  // channels per 16 byte piece
+  const int per_row = g.kb * 8;
+  for (int i = threadIdx.x; i < g.BN * per_row; i += (int)blockDim.x) {
+    const int n = i / per_row, j = i - n * per_row, blk = n / g.n1, k0 = j * E - blk * g.k1;
+    uint32_t v[4] = {0u, 0u, 0u, 0u};
+    if (n < g.N && k0 + E > 0 && k0 < g.k1) {
+      const uint8_t *w = g.w + (long long)(n - blk * g.n1) * g.ws;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (k0 + e >= 0 && k0 + e < g.k1) {
+          if (F8) v[e >> 2] |= (uint32_t)__ldg(w + k0 + e) << (8 * (e & 3));
+          else v[e >> 1] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(w) + k0 + e) << (16 * (e & 1));
+        }
+    }
+    sts128(wres + (uint32_t)(j >> 3) * step_bytes + (uint32_t)n * 128u + (uint32_t)(((j & 7) ^ (n & 7)) << 4),
+           make_uint4(v[0], v[1], v[2], v[3]));
+  }
+}
+
 // A warp's 32 staged rows (swizzled, 128 bytes apart) of `n` <= 64 channels from or to 32 packed rows, by 16 byte accesses.
 __device__ __forceinline__ __half *staged_at(uint8_t *stg, int r, int j) {
   return reinterpret_cast<__half *>(stg + r * 128 + ((((j >> 3) ^ (r & 7)) << 4) | ((j & 7) << 1)));
@@ -381,9 +408,31 @@ __device__ __forceinline__ void copy_packed(uint8_t *stg, __half *rows, int n, i
   }
 }
 
+// A NaN or an infinity in one row of a group reaches the others through the zeros of the block diagonal.  Sums that are not
+// finite are therefore taken again, each from its own row alone: channels [c, c + n) of grouped row `row`, over the staged
+// results.  (Rare, and slow: one thread, one channel after the other.)
+template <bool F8>
+__device__ __forceinline__ void redo_row(const LinArgs &g, uint8_t *stg_p, int lane, long long row, int c, int n) {
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    const int blk = (c + j) / g.n1, ch = c + j - blk * g.n1;
+    const uint8_t *x = g.x + row * g.xs + (long long)blk * g.k1 * (F8 ? 1 : 2), *w = g.w + (long long)ch * g.ws;
+    float acc = 0.0f;
+#pragma unroll 1
+    for (int k = 0; k < g.k1; ++k) {
+      if (F8) acc = fmaf(__half2float(__half(__nv_cvt_fp8_to_halfraw(x[k], __NV_E4M3))), __half2float(__half(__nv_cvt_fp8_to_halfraw(w[k], __NV_E4M3))), acc);
+      else acc = fmaf(__half2float(reinterpret_cast<const __half *>(x)[k]), __half2float(reinterpret_cast<const __half *>(w)[k]), acc);
+    }
+    float v[1] = {fmaf(acc, g.w_scale ? __ldg(g.w_scale + ch) : 1.0f, g.bias ? __half2float(__ldg(g.bias + ch)) : 0.0f)};
+    activate(v, g.act, g.alpha);
+    if (g.res) v[0] += __half2float(g.res[row * g.rs + c + j]);
+    *staged_at(stg_p, lane, j) = __float2half_rn(v[0]);
+  }
+}
+
 // NARROW: rows of out or of the residual may be ones that no tensor map takes; a kernel of its own, because the code for
 // them costs the others registers (frame 96 -> 64: 106 us without it, up to 129 with).
-template <int CG, bool F8, bool ANY, bool NARROW>
+template <int CG, bool F8, bool ANY, bool NARROW, bool GROUPED>
 __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_tile(const __grid_constant__ LinArgs g) {
   extern __shared__ uint8_t dyn[];
   const uint32_t base = aligned_base(dyn);
@@ -427,11 +476,16 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(hdr + HDR_TMEM);
   pdl_release();  // (after the allocation: blocks that wait for this kernel may hold tensor memory)
   pdl_wait();
+  if (GROUPED) {
+    fill_grouped<F8>(wres0, b_bytes, g);
+    fence_proxy_async();
+    __syncthreads();
+  }
 
   if (!ANY && warp == 0) {
     // ---- operand tiles by TMA; the pair's bytes are counted on the first block's barrier ----
     if (lane == 0) {
-      if (g.w_res) {
+      if (g.w_res && !GROUPED) {
         mbar_expect_tx(base + HDR_WRES, (uint32_t)g.kb * b_bytes);
         for (int kb = 0; kb < g.kb; ++kb)
           tma_load_2d<1>(wres0 + (uint32_t)kb * b_bytes, &g.tm_w, kb * (F8 ? 128 : 64), 0, base + HDR_WRES);
@@ -511,7 +565,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
       const uint32_t w0 = operand_desc(wres0), w_step = b_bytes >> 4;
       int s = 0, buf = 0;
       uint32_t ph = 0, bph = 1, a_s = a0;
-      bool ok = !g.w_res || warp_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
+      bool ok = !g.w_res || GROUPED || warp_wait(base + HDR_WRES, 0, abort_flag, g.status, 11);
       for (int t = first; ok && t < ntiles; t += step) {
         const uint32_t d = tmem + (uint32_t)(buf * g.BN);
         ok = warp_wait(base + HDR_TEMPTY + 8 * buf, bph, abort_flag, g.status, 14);
@@ -589,9 +643,9 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
         if (g.nt > 1 || g.BN > 64 || fresh)  // (else they are there from the team's first tile)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int j = lane + 32 * h, n = n0 + c + j;
-          col_b[j] = (g.bias && n < g.N) ? __half2float(__ldg(g.bias + n)) : 0.0f;
-          col_s[j] = (g.w_scale && n < g.N) ? __ldg(g.w_scale + n) : 1.0f;
+          const int j = lane + 32 * h, n = n0 + c + j, n1 = GROUPED ? n % g.n1 : n;
+          col_b[j] = (g.bias && n < g.N) ? __half2float(__ldg(g.bias + n1)) : 0.0f;
+          col_s[j] = (g.w_scale && n < g.N) ? __ldg(g.w_scale + n1) : 1.0f;
         }
         __syncwarp();
         if (g.res_tma) {
@@ -638,12 +692,17 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
+        float zero = 0.0f;  // (GROUPED: stays zero while every sum is finite)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (c + 32 * h >= nc) break;  // (uniform)
           uint32_t raw[32];
           tc_ld32(acc + (uint32_t)(c + 32 * h), raw);
           tc_wait_ld();
+          if (GROUPED) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) zero = fmaf(__uint_as_float(raw[i]), 0.0f, zero);
+          }
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
@@ -672,6 +731,7 @@ __global__ void __launch_bounds__(ANY ? ANY_THREADS : TILE_THREADS, 1) linear_ti
                                   pack_h2(v[8 * j + 4], v[8 * j + 5]), pack_h2(v[8 * j + 6], v[8 * j + 7])));
           }
         }
+        if (GROUPED && !(zero == 0.0f) && row < g.M) redo_row<F8>(g, stg_p, lane, row, c, min(64, nc - c));
         // (a store through the tensor map writes whole 16 byte pieces: not for a row that ends inside one)
         if (!NARROW || (g.out_tma && (c + 64 <= nc || (g.N & 7) == 0))) {
           fence_proxy_async();
@@ -1239,6 +1299,27 @@ int aligned_variant(long long rows, int n, int kb, int sms) {
 }
 int k_blocks(const Rec &r) { return (int)(((long long)r.d.c_in * r.es + 127) / 128); }
 
+// How many rows to take together as one (GROUPED), 1 for none: packed rows on a 16 byte boundary without scales of their
+// own, at most 256 channels out per group, the block diagonal of the weights within 96 KB, tiles for every SM.
+// 522240 rows 9 to 32 (leaky): 33 us through scratch, 20.8 grouped; 2088960 rows 3 to 16 91 and 27.8, 16 to 16 66 and 28.7.
+// Layers whose rows are on 16 byte boundaries as they are gain only where they are narrow: 32 to 32 20.5 and 18.8 (with
+// gelu and residual 43.7 and 46.9), 64 to 64 24.8 and 29.5.
+int group_rows(const Rec &r, int sms) {
+  const dnxcu_linear &d = r.d;
+  if (d.variant != DNXCU_LINEAR_AUTO || d.rows <= 16 || d.x_scale || d.x_stride != d.c_in || d.out_stride != d.c_out ||
+      (d.residual && d.residual_stride != d.c_out))
+    return 1;
+  if (((uintptr_t)d.x | (uintptr_t)d.out | (uintptr_t)d.residual) & 15) return 1;
+  if (fits_tc(r) && !(d.c_out & 7) && d.c_out > 24) return 1;
+  for (int g = 8; g > 1; g /= 2) {
+    const long long k = (long long)g * d.c_in * r.es, n = (long long)g * d.c_out;
+    if ((k & 15) || (n & 7) || n > 256) continue;
+    if ((k + 127) / 128 * ((n + 15) / 16 * 16) * 128 > 98304) continue;
+    if (d.rows / g >= 128ll * sms) return g;
+  }
+  return 1;
+}
+
 // The variant that runs the record.
 int pick(const Rec &r, int sms) {
   switch (r.d.variant) {
@@ -1248,6 +1329,7 @@ int pick(const Rec &r, int sms) {
     case DNXCU_LINEAR_ANY: return DNXCU_LINEAR_ANY;
     default: break;
   }
+  if (group_rows(r, sms) > 1) return DNXCU_LINEAR_TILE;
   if (!fits_tc(r)) return DNXCU_LINEAR_ANY;
   if (fits_rows(r)) return DNXCU_LINEAR_ROWS;
   return aligned_variant(r.d.rows, r.d.c_out, k_blocks(r), sms);
@@ -1260,6 +1342,9 @@ using namespace dnxcu;
 
 struct dnxcu_linear_plan {
   LinArgs a;
+  LinArgs tail;               // the last rows of a grouped layer, fewer than a group (tail_kernel: whether there are any)
+  const void *tail_kernel = nullptr;
+  dim3 tail_grid;
   RelayArgs relay;            // operands laid out anew in front of the kernel (scratch: where)
   void *scratch = nullptr;
   unsigned relay_grid = 0;
@@ -1286,7 +1371,8 @@ int sm_count(int dev) {
   return n;
 }
 
-#define TILE_KERNEL(cg, f8, any, narrow) (const void *)linear_tile<cg, f8, any, narrow>
+#define TILE_KERNEL(cg, f8, any, narrow) (const void *)linear_tile<cg, f8, any, narrow, false>
+#define GROUPED_KERNEL(f8) (const void *)linear_tile<1, f8, false, false, true>
 // Shared memory opt-in of every kernel, once per device.
 int init_device(int dev) {
   static std::atomic<int> done[kMaxDevices];
@@ -1294,7 +1380,8 @@ int init_device(int dev) {
   const void *k[] = {TILE_KERNEL(1, false, false, false), TILE_KERNEL(1, true, false, false), TILE_KERNEL(2, false, false, false),
                      TILE_KERNEL(2, true, false, false),  TILE_KERNEL(1, false, false, true), TILE_KERNEL(1, true, false, true),
                      TILE_KERNEL(2, false, false, true),  TILE_KERNEL(2, true, false, true),  TILE_KERNEL(1, false, true, true),
-                     TILE_KERNEL(1, true, true, true),    (const void *)linear_split<false>,  (const void *)linear_split<true>};
+                     TILE_KERNEL(1, true, true, true),    GROUPED_KERNEL(false),              GROUPED_KERNEL(true),
+                     (const void *)linear_split<false>,   (const void *)linear_split<true>};
   for (const void *f : k) DNXCU_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit));
   if (dev < kMaxDevices) done[dev].store(1, std::memory_order_release);
   return DNXCU_OK;
@@ -1302,7 +1389,7 @@ int init_device(int dev) {
 
 void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   LinArgs &a = p->a;
-  const TileShape shape = pick_tile(a.M, a.N, a.kb, sms, any);
+  const TileShape shape = a.gr > 1 ? TileShape{round_up(a.N, 16), 1, 0.0} : pick_tile(a.M, a.N, a.kb, sms, any);
   const int bn = shape.bn, cg = shape.cg;
   // The weights pass through L2 once per group of rows, so a group is as many rows as keep 36 MB of x (of 126 MB of L2)
   // in flight, 4 to 32 tiles.  Under the power limit 8192 x 4096 x 16384 binary16 takes 867, 848, 940 us with groups of 8,
@@ -1319,7 +1406,7 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   const bool narrow = !mappable(r.d.out, a.os * 2) || (r.d.residual && !mappable(r.d.residual, a.rs * 2));
   a.teams = a.kb >= 16 && !any && !(narrow && a.kb < 32 && (long long)a.mt * a.nt > sms / cg) ? 1 : 2;
   const uint32_t wbytes = (uint32_t)(bn / cg) * 128u;
-  a.w_res = cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536;
+  a.w_res = a.gr > 1 || (cg == 1 && a.nt == 1 && a.mt > sms && (long long)a.kb * wbytes <= 65536);
   const uint32_t fixed = 1024u + TILE_FIXED + 4u * (uint32_t)a.teams * STAGING + (a.w_res ? (uint32_t)a.kb * wbytes : 0u);
   // Two steps per stage where three such stages fit: half the waits and commits of the issuing warp, which is what bounds
   // tiles of up to 128 channels.
@@ -1335,7 +1422,8 @@ void plan_tile(const Rec &r, int sms, bool any, dnxcu_linear_plan *p) {
   p->block = dim3(any ? ANY_THREADS : TILE_THREADS);
   p->cluster = (uint32_t)cg;
   const bool tail = narrow || (a.N & 7);  // (a row that ends inside 16 bytes: see the store)
-  if (any) p->kernel = r.f8 ? TILE_KERNEL(1, true, true, true) : TILE_KERNEL(1, false, true, true);
+  if (a.gr > 1) p->kernel = r.f8 ? GROUPED_KERNEL(true) : GROUPED_KERNEL(false);
+  else if (any) p->kernel = r.f8 ? TILE_KERNEL(1, true, true, true) : TILE_KERNEL(1, false, true, true);
   else if (cg == 2 && tail) p->kernel = r.f8 ? TILE_KERNEL(2, true, false, true) : TILE_KERNEL(2, false, false, true);
   else if (cg == 2) p->kernel = r.f8 ? TILE_KERNEL(2, true, false, false) : TILE_KERNEL(2, false, false, false);
   else if (tail) p->kernel = r.f8 ? TILE_KERNEL(1, true, false, true) : TILE_KERNEL(1, false, false, true);
@@ -1403,7 +1491,7 @@ int plan_kernel(const Rec &r, int v, const void *x, const void *w, int sms, dnxc
   plan_tile(r, sms, v == DNXCU_LINEAR_ANY, p);
   if (v == DNXCU_LINEAR_TILE) {
     st = matrix_map(&a.tm_x, x, r.f8, a.M, a.K, a.xs, 128);
-    if (!st) st = matrix_map(&a.tm_w, w, r.f8, a.N, a.K, a.ws, a.BN / (int)p->cluster);
+    if (!st && a.gr == 1) st = matrix_map(&a.tm_w, w, r.f8, a.N, a.K, a.ws, a.BN / (int)p->cluster);
     if (st) return st;
   }
   a.out_tma = mappable(d.out, a.os * 2);
@@ -1459,6 +1547,32 @@ int make_plan(const Rec &r, dnxcu_linear_plan *p, bool keep) {
   a.status = d.device_status;
   a.wait_limit = wait_limit_cycles();
   if (a.wait_limit < 2000000ull) a.wait_limit |= 1ull << 63;  // below about a millisecond: strict (see mbar_wait)
+  a.gr = 1;
+  if (const int gr = v == DNXCU_LINEAR_TILE ? group_rows(r, sms) : 1; gr > 1) {
+    const int left = a.M % gr;
+    if (left) {
+      p->tail = a;
+      LinArgs &t = p->tail;
+      t.M = left;
+      const long long r0 = a.M - left;
+      t.x = (const uint8_t *)d.x + r0 * a.xs;
+      t.w = (const uint8_t *)d.weights;
+      t.out += r0 * a.os;
+      if (t.res) t.res += r0 * a.rs;
+      p->tail_kernel = r.f8 ? (const void *)linear_rows<true, 1, 1, 1, true> : (const void *)linear_rows<false, 1, 1, 1, true>;
+      p->tail_grid = dim3((unsigned)((a.N + 15) / 16));
+    }
+    a.gr = gr;
+    a.n1 = a.N;
+    a.k1 = a.K;
+    a.M /= gr;
+    a.N *= gr;
+    a.K *= gr;
+    a.xs *= gr;
+    a.rs *= gr;
+    a.os *= gr;
+    a.kb = (a.K * r.es + 127) / 128;
+  }
   // Unaligned operands of a kept plan: laid out anew in scratch memory by one kernel, then the aligned variants.
   if (v == DNXCU_LINEAR_ANY && d.variant == DNXCU_LINEAR_AUTO && keep && a.M > 16) {
     RelayArgs &y = p->relay;
@@ -1503,6 +1617,10 @@ int launch(const dnxcu_linear_plan &p, cudaStream_t s) {
   }
   void *args[] = {const_cast<LinArgs *>(&p.a)};
   DNXCU_CUDA(launch_dependent(p.kernel, p.grid, p.block, p.smem, p.cluster, s, args));
+  if (p.tail_kernel) {
+    void *targs[] = {const_cast<LinArgs *>(&p.tail)};
+    DNXCU_CUDA(launch_dependent(p.tail_kernel, p.tail_grid, dim3(ROWS_THREADS), 0, 1, s, targs));
+  }
   return DNXCU_OK;
 }
 

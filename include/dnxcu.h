@@ -328,7 +328,8 @@ typedef enum dnxcu_linear_variant {
                              boundaries, row strides and c_in multiples of 16 bytes */
   DNXCU_LINEAR_SPLIT = 2, /* few rows on the tensor cores: c_in split over the blocks of a cluster; x and weights on 16
                              byte boundaries with row strides that are multiples of 16 bytes */
-  DNXCU_LINEAR_TILE = 3,  /* tiles of rows on the tensor cores; x and weights as for SPLIT */
+  DNXCU_LINEAR_TILE = 3,  /* tiles of rows on the tensor cores; x and weights as for SPLIT (AUTO also takes it for thin
+                             layers over many packed rows of any length, several rows at a time) */
   DNXCU_LINEAR_ANY = 4    /* ROWS and TILE with operands fetched by plain loads: any alignment, any stride */
 } dnxcu_linear_variant;
 

@@ -56,6 +56,9 @@ def reference(x, w, xs=None, ws=None, bias=None, residual=None, act="none"):
     k = x.shape[1]
     tol = 1.2 * (k + 32) * 2.0 ** -23 * (mag + (z - s * scale).abs()) + y.abs() * (16 + 2 * z.abs()) * 2.0 ** -23 \
         + z.abs() * 2.0 ** -22 + (out.abs() + y.abs()) * 2.0 ** -24 + out.abs() * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25
+    # An infinite sum has no error, and an activation that is finite there is so exactly (relu of minus infinity is 0): what
+    # is left is the residual's addition to that value and the output's rounding.
+    tol = torch.where(torch.isinf(z) & torch.isfinite(out), out.abs() * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25, tol)
     return out.cpu(), tol.cpu()
 
 
@@ -261,6 +264,43 @@ def test_plan_of_unaligned_operands(m, k, n, strides, offsets, dtype):
     for planned in (True, False):
         got = run(x, w, xs, ws, b, r, "silu", strides=strides + (0, 0), offsets=offsets + (0, 0), planned=planned)
         assert_within(got, ref, tol, f"planned={planned}")
+
+
+# (rows, c_in, c_out, dtype) that AUTO takes several rows at a time: 8, 8 with rows left over, 2, 4, 8 bit operands
+GROUPED = [(151552, 9, 32, "f16"), (151560 + 5, 9, 32, "f16"), (160003, 3, 16, "f16"), (152001, 3, 9, "f16"), (39999, 8, 8, "f16"),
+           (76003, 12, 20, "f16"), (155555, 16, 16, "f16"), (151557, 27, 5, "f16"), (151999, 2, 8, "e4m3"), (160000, 30, 9, "e4m3")]
+
+
+@pytest.mark.parametrize("m,k,n,dtype", GROUPED)
+def test_thin_layers_over_many_rows(m, k, n, dtype):
+    t = torch.float16 if dtype == "f16" else torch.float8_e4m3fn
+    g = torch.Generator().manual_seed(m)
+    x, w = torch.randint(-2, 3, (m, k), generator=g).to(t), torch.randint(-2, 3, (n, k), generator=g).to(t)
+    bias, r = torch.randint(-8, 9, (n,), generator=g).half(), torch.randint(-100, 101, (m, n), generator=g).half()
+    want = x.double() @ w.double().t() + bias.double() + r.double()
+    for in_place in (False, True):
+        assert torch.equal(run(x, w, bias=bias, residual=r, in_place=in_place), want)
+    assert torch.equal(run(x, w, bias=bias, planned=True), want - r.double())
+    ws = 0.5 + torch.rand(n, generator=g)
+    x = normal(m, m, k, dtype=torch.float32).to(t)
+    ref, tol = reference(x, w, ws=ws, bias=bias, act="gelu")
+    assert_within(run(x, w, ws=ws, bias=bias, act="gelu"), ref, tol)
+
+
+@pytest.mark.parametrize("m,k,n,dtype", GROUPED)
+def test_thin_layers_keep_values_that_are_not_finite_in_their_row(m, k, n, dtype):
+    t = torch.float16 if dtype == "f16" else torch.float8_e4m3fn
+    x, w = normal(1, m, k, dtype=torch.float32).to(t), normal(2, n, k, dtype=torch.float32)
+    w[:, 0] = w[:, 0].abs() + 0.5
+    w = w.to(t)
+    bias, r = normal(3, n), normal(4, m, n)
+    for i, v in ((0, "nan"), (13, "inf"), (14, "-inf"), (m // 2, "nan"), (m - 1, "inf")):
+        x[i, 0] = float(v) if dtype == "f16" else float("nan")
+    for act in ("none", "relu"):
+        ref, tol = reference(x, w, bias=bias, residual=r, act=act)
+        got = run(x, w, bias=bias, residual=r, act=act)
+        assert_within(got, ref, tol, act)
+        assert_within(run(x, w, bias=bias, residual=r, act=act, in_place=True), ref, tol, act)
 
 
 def test_offsets_past_32_bits():

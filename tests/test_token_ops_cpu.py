@@ -76,6 +76,11 @@ def test_linear_accepts_and_picks():
     assert pick(c_in=65) == lib.LINEAR_ANY and pick(x=X + 2) == lib.LINEAR_ANY and pick(weights=W + 8) == lib.LINEAR_ANY
     assert pick(c_in=65, x_stride=72, w_stride=80) != lib.LINEAR_ANY  # padded rows
     assert pick(dtype=lib.DT_E4M3, c_in=72) == lib.LINEAR_ANY
+    # thin layers over many packed rows: several at a time, whatever the alignment of a single one
+    thin = dict(rows=522240, c_in=9, c_out=32, x_scale=None, residual=None, out=0x100000000)
+    assert pick(**thin) == lib.LINEAR_TILE
+    for kw in (dict(x_stride=10), dict(out_stride=40), dict(x_scale=XS), dict(rows=1000), dict(x=X + 2), dict(c_out=40)):
+        assert pick(**{**thin, **kw}) == lib.LINEAR_ANY
     assert pick(residual=None, bias=None, x_scale=None, w_scale=None, rows=1, c_in=1, c_out=1) == lib.LINEAR_ANY
     assert pick(residual=O) > 0  # in place
     for v, kw in ((lib.LINEAR_ROWS, dict(rows=16)), (lib.LINEAR_SPLIT, {}), (lib.LINEAR_TILE, {}), (lib.LINEAR_ANY, {})):
