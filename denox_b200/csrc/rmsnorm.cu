@@ -7,8 +7,10 @@
 // One pass over the data: a row's elements stay in registers between the statistics and the output.  The row's
 // largest |y| needs no second reduction: 1 / rms is a positive constant of the row, so max|y| = max|weight * h| / rms
 // is taken beside the sum of squares, and q = (weight * h) * (448 / max|weight * h|) does not need rms at all.
-// The maximum is taken on the absolute values' bit patterns, whose unsigned order is the values' order with NaN
-// above infinity: a row that is not finite shows in it, and one integer `redux` does a warp's.
+// The maximum carries a NaN along, so a row that is not finite shows in it; across threads it is taken on the bit patterns,
+// whose unsigned order is the values' order with NaN above infinity: one integer `redux` does a warp's.
+// With an 8 bit output weight * h takes h's place in the registers as soon as the sum is stored: one product and one fetch of
+// the weights per element instead of two, which is power, and that is clock (1000 W are reached by this kernel too).
 //
 // Bound by bytes: 16384 rows of 4096 with residual to e4m3 72.5 us (6.5 TB/s), 2088960 rows of 32 43.8 us (6.1 TB/s).  Six
 // forms, by the row's length and by what the alignment allows (V elements per access, 16 bytes
@@ -48,7 +50,12 @@ union Halves {
   __half h[V];
 };
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// max(a, |b|), NaN when either is: the largest value of a row also tells whether all of it is finite.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
 
 // Loads of data that an output of the same call may alias are plain loads (never the read-only path); every thread
 // reads an element before it writes it, and no thread reads another's.
@@ -120,14 +127,14 @@ template <int V>
 __device__ __forceinline__ void store_sum(const NormArgs &g, long long row, int c, const float (&h)[V]) {
   store_halves<V>(g.sum + row * g.ss + c, h);
 }
-// y = weight * h * f, rounded once to the output type.  8 bits: f = 448 / max|weight * h|; a product that the last
-// bit of f puts above 448 saturates to it.
+// y = weight * h * f, rounded once to the output type.  8 bits: `h` is weight * h already and f = 448 / max|weight * h|; a
+// product that the last bit of f puts above 448 saturates to it.
 template <int V, bool Q>
 __device__ __forceinline__ void store_out(const NormArgs &g, long long row, int c, const float (&h)[V], const float (&w)[V],
                                           float f) {
   float y[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) y[e] = Q ? h[e] * w[e] * f : h[e] * f * w[e];
+  for (int e = 0; e < V; ++e) y[e] = Q ? h[e] * f : h[e] * f * w[e];
   if constexpr (!Q) {
     store_halves<V>((__half *)g.out + row * g.os + c, y);
   } else if constexpr (V == 1) {
@@ -191,17 +198,22 @@ __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float h[N][V], ss = 0.0f;
-      uint32_t top = 0;
+      float h[N][V], ss = 0.0f, most = 0.0f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
+        const int vi = t + (i << lt);
         sum_raw<V, RES>(raw[u][i], h[i]);
+        if (g.sum && row[u] < g.rows && vi < nv) store_sum<V>(g, row[u], vi * V, h[i]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           ss = fmaf(h[i][e], h[i][e], ss);
-          if (Q) top = max(top, abs_bits(h[i][e] * w[i][e]));
+          if (Q) {
+            h[i][e] *= w[i][e];
+            most = max_abs(most, h[i][e]);
+          }
         }
       }
+      uint32_t top = __float_as_uint(most);
       for (int o = tpr >> 1; o > 0; o >>= 1) {
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (Q) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -213,10 +225,7 @@ __global__ void __launch_bounds__(256) rmsnorm_warp(NormArgs g, int lt) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int vi = t + (i << lt);
-        if (vi < nv) {
-          if (g.sum) store_sum<V>(g, row[u], vi * V, h[i]);
-          store_out<V, Q>(g, row[u], vi * V, h[i], w[i], f);
-        }
+        if (vi < nv) store_out<V, Q>(g, row[u], vi * V, h[i], w[i], f);
       }
     }
   }
@@ -253,22 +262,25 @@ __global__ void __launch_bounds__(1024) rmsnorm_block(NormArgs g) {
     Raw<V, RES> raw[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) load_raw<V, RES>(g, row, (t + i * nt) * V, t + i * nt < nv, raw[i]);
-    float h[N][V];
-#pragma unroll
-    for (int i = 0; i < N; ++i) sum_raw<V, RES>(raw[i], h[i]);
-    float ss = 0.0f;
-    uint32_t top = 0;
+    float h[N][V], ss = 0.0f, most = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float w[V];
       const int vi = t + i * nt;
-      if (Q && vi < nv) load_weight<V>(g, vi * V, w);
+      sum_raw<V, RES>(raw[i], h[i]);
+      if (g.sum && vi < nv) store_sum<V>(g, row, vi * V, h[i]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        ss = fmaf(h[i][e], h[i][e], ss);
-        if (Q && vi < nv) top = max(top, abs_bits(h[i][e] * w[e]));
+      for (int e = 0; e < V; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+      if (Q && vi < nv) {
+        float w[V];
+        load_weight<V>(g, vi * V, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          h[i][e] *= w[e];
+          most = max_abs(most, h[i][e]);
+        }
       }
     }
+    uint32_t top = __float_as_uint(most);
     block_reduce(ss, top, turn);
     float scale = 0.0f;
     const float f = row_factor<Q>(g, ss, top, &scale);
@@ -278,8 +290,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_block(NormArgs g) {
       const int vi = t + i * nt;
       if (vi < nv) {
         float w[V];
-        load_weight<V>(g, vi * V, w);  // (from L1: every row uses the same ones)
-        if (g.sum) store_sum<V>(g, row, vi * V, h[i]);
+        if (!Q) load_weight<V>(g, vi * V, w);  // (from L1: every row uses the same ones)
         store_out<V, Q>(g, row, vi * V, h[i], w, f);
       }
     }
@@ -361,8 +372,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_shift(NormArgs g, i
         w[2 * e + 1] = f.y;
       }
     };
-    float h[N][8], ss = 0.0f;
-    uint32_t top = 0;
+    float h[N][8], ss = 0.0f, most = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       Raw<8, RES> raw;
@@ -370,14 +380,30 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_shift(NormArgs g, i
       if (RES) raw.r = vr[i];
       sum_raw<8, RES>(raw, h[i]);
       const int k = t + i * nt, c = 8 * k - lead;
-      float w[8];
-      if (Q && k < words) weight(k, c, w);
+      if (g.sum && k < words) {
+        if (c >= 0 && c + 8 <= g.C) {
+          store_sum<8>(g, row, c, h[i]);
+        } else {
+          __half v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ss = fmaf(h[i][e], h[i][e], ss);
-        if (Q && k < words) top = max(top, abs_bits(h[i][e] * w[e]));
+          for (int e = 0; e < 8; ++e) v[e] = __float2half_rn(h[i][e]);
+          store_edge(g.sum + row * g.ss, c, g.C, v);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+      if (Q && k < words) {
+        float w[8];
+        weight(k, c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // (an element of the word that is not the row's is 0 and has weight 0, or 1 without weights)
+          h[i][e] *= w[e];
+          most = max_abs(most, h[i][e]);
+        }
       }
     }
+    uint32_t top = __float_as_uint(most);
     if (WARP) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -393,24 +419,14 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_shift(NormArgs g, i
       const int k = t + i * nt, c = 8 * k - lead;
       if (k >= words) continue;
       const bool all = c >= 0 && c + 8 <= g.C;
-      if (g.sum) {
-        if (all) {
-          store_sum<8>(g, row, c, h[i]);
-        } else {
-          __half v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = __float2half_rn(h[i][e]);
-          store_edge(g.sum + row * g.ss, c, g.C, v);
-        }
-      }
       float w[8];
-      weight(k, c, w);
+      if (!Q) weight(k, c, w);
       if (all) {
         store_out<8, Q>(g, row, c, h[i], w, f);
       } else if (Q) {
         uint8_t v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (uint8_t)pack_e4m3(h[i][e] * w[e] * f, 0.0f);
+        for (int e = 0; e < 8; ++e) v[e] = (uint8_t)pack_e4m3(h[i][e] * f, 0.0f);
         store_edge((uint8_t *)g.out + row * g.os, c, g.C, v);
       } else {
         __half v[8];
@@ -463,14 +479,14 @@ __global__ void __launch_bounds__(256) rmsnorm_packed(NormArgs g, int group, int
     __syncthreads();
     const int lanes = 1 << log_lanes, l = t & (lanes - 1);
     for (int q = t >> log_lanes; q < ((rows + (256 >> log_lanes) - 1) & ~((256 >> log_lanes) - 1)); q += 256 >> log_lanes) {
-      float ss = 0.0f;
-      uint32_t top = 0;
+      float ss = 0.0f, most = 0.0f;
       if (q < rows)
         for (int j = l; j < C; j += lanes) {
           const float v = s_h[q * C + j];
           ss = fmaf(v, v, ss);
-          if (Q) top = max(top, abs_bits(v * s_w[j]));
+          if (Q) most = max_abs(most, v * s_w[j]);
         }
+      uint32_t top = __float_as_uint(most);
       for (int o = lanes >> 1; o > 0; o >>= 1) {
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (Q) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
   int turn = 0;
   for (long long row = blockIdx.x; row < g.rows; row += gridDim.x, turn ^= 1) {
     double sum = 0.0;  // (a thread may add thousands of terms one after the other)
-    uint32_t top = 0;
+    float most = 0.0f;
 #pragma unroll 4
     for (int vi = t; vi < nv; vi += nt) {
       float h[V], w[V];
@@ -545,11 +561,12 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         ss = fmaf(h[e], h[e], ss);
-        if (Q) top = max(top, abs_bits(h[e] * w[e]));
+        if (Q) most = max_abs(most, h[e] * w[e]);
       }
       sum += ss;
     }
     float ss = (float)sum;
+    uint32_t top = __float_as_uint(most);
     block_reduce(ss, top, turn);
     float scale = 0.0f;
     const float f = row_factor<Q>(g, ss, top, &scale);
@@ -562,6 +579,10 @@ __global__ void __launch_bounds__(1024) rmsnorm_loop(NormArgs g) {
       sum_raw<V, RES>(raw, h);
       load_weight<V>(g, vi * V, w);
       if (g.sum) store_sum<V>(g, row, vi * V, h);
+      if (Q) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[e] *= w[e];
+      }
       store_out<V, Q>(g, row, vi * V, h, w, f);
     }
   }
