@@ -15,7 +15,7 @@
 // Bound by bytes: 16384 rows of 4096 with residual to e4m3 72.5 us (6.5 TB/s), 2088960 rows of 32 43.8 us (6.1 TB/s).  Six
 // forms, by the row's length and by what the alignment allows (V elements per access, 16 bytes
 // where every pointer and stride is a multiple of that):
-//   warp form  rows of at most 1024 channels: a power of two of lanes per row, several rows per warp; every thread
+//   warp form  rows of at most 512 channels: a power of two of lanes per row, several rows per warp; every thread
 //              has 32 elements in flight whatever the row's length (U rows of E elements, U * E = 32);
 //   block form rows up to 32 elements x 1024 threads: a block per row;
 //   shifted form  rows off 16 byte boundaries, but all tensors of the call alike: 16 byte accesses inside the row, single
@@ -600,17 +600,16 @@ cudaError_t launch_v(const NormArgs &g, cudaStream_t s) {
     void *args[] = {const_cast<NormArgs *>(&g), &lt};  // (only the warp form takes the second)
     return cudaLaunchKernel(kernel, dim3(grid), dim3((unsigned)threads), args, 0, s);
   };
-  if (g.C <= 1024) {
-    // the fewest lanes (a power of two) that hold the row in 8, 16 or 32 elements per thread, most rows per warp first
-    const int e = g.C <= 256 ? 8 : g.C <= 512 ? 16 : 32;
+  if (g.C <= 512) {
+    // the fewest lanes (a power of two) that hold the row in 8 or 16 elements per thread, most rows per warp first (with 32,
+    // up to 1024 channels, the registers leave too few warps: 50000 rows of 1024 52.8 us, 34.6 in the block form)
+    const int e = g.C <= 256 ? 8 : 16;
     int lt = 0;
     while ((e / V) << lt < nv) ++lt;
     const long long per_block = (256 >> lt) * (32 / e);
     const long long blocks = (g.rows + per_block - 1) / per_block;
     const unsigned grid = (unsigned)(blocks < kMaxGrid ? blocks : kMaxGrid);
-    if (e == 8) return enqueue((const void *)rmsnorm_warp<V, 8, Q, RES>, grid, 256, lt);
-    if (e == 16) return enqueue((const void *)rmsnorm_warp<V, 16, Q, RES>, grid, 256, lt);
-    return enqueue((const void *)rmsnorm_warp<V, 32, Q, RES>, grid, 256, lt);
+    return enqueue(e == 8 ? (const void *)rmsnorm_warp<V, 8, Q, RES> : (const void *)rmsnorm_warp<V, 16, Q, RES>, grid, 256, lt);
   }
   const unsigned grid = (unsigned)(g.rows < kMaxGrid ? g.rows : kMaxGrid);
   const auto threads = [&](int e) {
@@ -638,10 +637,8 @@ cudaError_t launch_shift(const NormArgs &g, cudaStream_t s) {
   void *args[] = {const_cast<NormArgs *>(&g), &aligned};
   const int words = (g.C + 14) / 8;  // of the widest row
   const auto blocks = [](long long n) { return dim3((unsigned)(n < kMaxGrid ? n : kMaxGrid)); };
-  if (words <= 128) {
-    const void *k = words <= 32   ? (const void *)rmsnorm_shift<8, Q, RES, true>
-                    : words <= 64 ? (const void *)rmsnorm_shift<16, Q, RES, true>
-                                  : (const void *)rmsnorm_shift<32, Q, RES, true>;
+  if (words <= 64) {
+    const void *k = words <= 32 ? (const void *)rmsnorm_shift<8, Q, RES, true> : (const void *)rmsnorm_shift<16, Q, RES, true>;
     return cudaLaunchKernel(k, blocks((g.rows + 7) / 8), dim3(256), args, 0, s);
   }
   const bool few = g.rows <= 148;
@@ -771,7 +768,9 @@ int dnxcu_rmsnorm_launch(const dnxcu_rmsnorm *d, void *stream) {
     return !((uintptr_t)g.out & ob) && g.os % v == 0;
   };
   cudaStream_t s = (cudaStream_t)stream;
-  if (!fits(8) && g.C >= kShiftFrom && g.C <= 32768 - 14 && same_lead(g, q)) {
+  // (up to 1024 channels narrower accesses beat it where they are wider than one element: 50000 rows of 516: 49 against 38
+  // us, of 1022 80 against 61; 16384 of 4098: 74 against 91, of 4100 with residual to e4m3 101 against 134)
+  if (!fits(g.C <= 1024 ? 2 : 8) && g.C >= kShiftFrom && g.C <= 32768 - 14 && same_lead(g, q)) {
     const auto run = q ? (g.residual ? launch_shift<true, true> : launch_shift<true, false>)
                        : (g.residual ? launch_shift<false, true> : launch_shift<false, false>);
     DNXCU_CUDA(run(g, s));
