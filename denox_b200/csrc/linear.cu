@@ -1291,7 +1291,9 @@ SplitShape pick_split(long long rows, int n, int kb, int sms) {
   while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= kb) p.split *= 2;
   if (p.split < 8 && kb / p.split >= 64) p.split *= 2;
   const double waves = (double)((tiles * p.split + sms - 1) / sms);
-  p.us = 4.0 + 0.03 * p.bn + waves * ((kb + p.split - 1) / p.split) * (0.34 + (p.bn > 128 ? (p.bn - 128) * 0.0012 : 0.0));
+  // (set-up and join are paid by every wave, but for two small blocks that share an SM; 2032 x 112 x 11072: five waves, 63 us)
+  const double fixed = (waves <= 2.0 && p.bn <= 64 ? 1.0 : waves) * (4.0 + 0.03 * p.bn);
+  p.us = fixed + waves * ((kb + p.split - 1) / p.split) * (0.34 + (p.bn > 128 ? (p.bn - 128) * 0.0012 : 0.0));
   return p;
 }
 int aligned_variant(long long rows, int n, int kb, int sms) {
