@@ -121,3 +121,50 @@ def test_every_kernel_at_once_on_three_streams():
     for chain in chains:
         for plan, *_ in chain:
             plan.close()
+
+
+def test_capture_with_a_fork_and_a_join():
+    """Two layers on forked streams between two others, captured into one graph: every edge holds."""
+    half = dict(dtype=torch.float16, device="cuda")
+    p = lambda t: t.data_ptr()
+    m, c = 700, 512
+    x, w = normal(1, m, c).cuda(), [normal(2 + i, c, c, scale=1 / math.sqrt(c)).cuda() for i in range(4)]
+    a, b1, b2, out = (torch.empty(m, c, **half) for _ in range(4))
+    layer = lambda src, i, dst, res=None: lib.LinearPlan(lib.linear_desc(m, c, c, p(src), p(w[i]), p(dst), residual=p(res) if res is not None else None))
+    plans = [layer(x, 0, a), layer(a, 1, b1), layer(a, 2, b2), layer(b1, 3, out, b2)]
+    for q in plans:
+        q.launch()
+        torch.cuda.synchronize()
+    want = [t.clone() for t in (a, b1, b2, out)]
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        main = torch.cuda.current_stream()
+        plans[0].launch(main.cuda_stream)
+        side.wait_stream(main)
+        plans[1].launch(main.cuda_stream)
+        plans[2].launch(side.cuda_stream)
+        main.wait_stream(side)
+        plans[3].launch(main.cuda_stream)
+    for _ in range(10):
+        for t in (a, b1, b2, out):
+            t.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, v) for t, v in zip((a, b1, b2, out), want))
+    # and without a graph
+    for _ in range(10):
+        for t in (a, b1, b2, out):
+            t.fill_(float("nan"))
+        main = torch.cuda.current_stream()
+        plans[0].launch(main.cuda_stream)
+        side.wait_stream(main)
+        plans[1].launch(main.cuda_stream)
+        plans[2].launch(side.cuda_stream)
+        main.wait_stream(side)
+        plans[3].launch(main.cuda_stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, v) for t, v in zip((a, b1, b2, out), want))
+    del g
+    for q in plans:
+        q.close()
