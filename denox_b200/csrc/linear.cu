@@ -895,15 +895,15 @@ __global__ void __launch_bounds__(SPLIT_THREADS) linear_split(const __grid_const
       tc_ld16(tmem + (uint32_t)c + ((uint32_t)(q * 32) << 16), raw);
       tc_wait_ld();
       int to = c / per, r = c - to * per;
+      const uint32_t mine0 = recv + (uint32_t)(rank * per * 128 + q * 32 + lane) * 4u;
+      uint32_t dst = map_rank(mine0, (uint32_t)to) + (uint32_t)r * 512u;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if (c + i < rows) {
-          const uint32_t at = recv + (uint32_t)((rank * per + r) * 128 + q * 32 + lane) * 4u;
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_rank(at, (uint32_t)to)), "r"(raw[i]) : "memory");
-        }
-        if (++r == per) {
+        if (c + i < rows) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(raw[i]) : "memory");
+        dst += 512u;
+        if (++r == per && c + i + 1 < rows) {
           r = 0;
-          ++to;
+          dst = map_rank(mine0, (uint32_t)++to);
         }
       }
     }
