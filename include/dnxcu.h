@@ -256,8 +256,9 @@ DNXCU_API int dnxcu_conv3x3_pool_static(const void *in, int height, int width, i
  *    own length).  Rows may be windows of wider rows (stride > length);
  *  - the entry points check the record before anything is enqueued:
  *    DNXCU_E_BAD_ARG (null pointer, non-positive size, unknown enum, stride
- *    below the row length, operands that overlap where they may not, a buffer
- *    that the current device does not hold), DNXCU_E_MISALIGNED (a pointer
+ *    below the row length, operands that overlap where they may not - rows
+ *    that interleave count unless both have one stride -, a buffer that the
+ *    current device does not hold), DNXCU_E_MISALIGNED (a pointer
  *    that is not a multiple of its element), DNXCU_E_LIMIT (a size above the
  *    limits below), DNXCU_E_UNSUPPORTED (a forced variant that cannot run it);
  *  - launches are stream ordered, never synchronise, allocate nothing, keep
